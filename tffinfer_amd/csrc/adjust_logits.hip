@@ -1,0 +1,147 @@
+// What the requests' options do to rows of logits before a token is chosen: penalties for tokens that the request has seen, biases of
+// single tokens, a mask of the tokens that a grammar allows.  For token v of a row,
+//   x <- x > 0 ? x / rep : x * rep            if v stands in the request's prompt or output (what tff_repetition_penalty does)
+//   x <- x - freq n_v - pres [n_v > 0]        n_v: how often v stands in its output
+//   x <- x + bias_v                           if v is listed
+//   x <- -inf                                 where the row's mask has no bit
+// The rows of drafted trees' nodes belong to the tree's request and have the tokens on their path (`ancestors`) as output besides.
+// The reference has the first of these, on the host (src/core/sampler/LLMSampler.cpp:21-34).
+//
+// A block takes a run of the vocabulary of one row and counts the tokens of the request's whole history that fall into it in LDS: the
+// history comes as it is, with repetitions, no table of counts by token has to be kept or cleared, counts are integers and so
+// do not depend on the order of the atomics.  Then it goes over its run once: what is masked is written and not read, and in place what no
+// option touches is neither.  The bound is memory: 4 bytes a logit in and out.
+#include "common.h"
+#include "tffinfer_kernels.h"
+
+#define ADJUST_SEEN 0x80000000u      // in the prompt; the bits below count the output
+
+struct AdjustArgs {
+    const float* logits;
+    float* out;
+    int rows, V, runs;
+    const int32_t *history, *cu_history, *prompt_lens;
+    int history_len, requests;
+    const float *repetition, *presence, *frequency;
+    const int32_t* bias_ids;
+    const float* bias_values;
+    const int32_t* cu_bias;
+    int bias_len;
+    const int32_t* masks;
+    int num_masks, mask_words;
+    const int32_t* mask_rows;
+    const int32_t *draft_tokens, *cu_nodes, *ancestors;
+    int words;
+};
+
+// The request that row t belongs to, the same in every lane: as many of cu[1 .. n] as are not behind t (n: to none).
+__device__ __forceinline__ int row_request(const int32_t* __restrict__ cu, int n, int t) {
+    int upto = 0;
+    for (int r0 = 0; r0 < n; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        upto += __popcll(__ballot(r < n && cu[min(r, n - 1) + 1] <= t));
+    }
+    return upto;
+}
+
+template <int RUN>
+__global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) {
+    __shared__ uint32_t cnt[RUN];
+    const int t = blockIdx.x / a.runs, v0 = (blockIdx.x - t * a.runs) * RUN, n = min(RUN, a.V - v0), tid = threadIdx.x;
+    const size_t base = (size_t)t * a.V + v0;
+    const float* __restrict__ x = a.logits + base;
+    float* __restrict__ y = a.out + base;
+    const bool in_place = a.logits == a.out;
+    int r = t;
+    if (a.cu_nodes) r = row_request(a.cu_nodes, a.requests, t);
+    const bool has_request = r < a.requests;      // (a row behind the last node is left as it is)
+    const int mask_row = a.mask_rows ? a.mask_rows[t] : -1;
+    const int32_t* __restrict__ mask = has_request && mask_row >= 0 && mask_row < a.num_masks ? a.masks + (size_t)mask_row * a.mask_words : nullptr;
+    float rep = 1.f, pres = 0.f, freq = 0.f;
+    if (has_request) {
+        rep = a.repetition[r];
+        pres = a.presence[r];
+        freq = a.frequency[r];
+    }
+    const bool counts = rep != 1.f || pres != 0.f || freq != 0.f;
+    if (counts) {
+        for (int i = tid; i < n; i += 256) cnt[i] = 0;
+        __syncthreads();
+        const int h0 = min(max(a.cu_history[r], 0), a.history_len), h1 = min(max(a.cu_history[r + 1], h0), a.history_len);
+        const int out0 = h0 + min(max(a.prompt_lens[r], 0), h1 - h0);
+        for (int i = h0 + tid; i < h1; i += 256) {
+            const int at = a.history[i] - v0;
+            if (at >= 0 && at < n) {
+                if (i < out0) atomicOr(&cnt[at], ADJUST_SEEN);
+                else atomicAdd(&cnt[at], 1u);
+            }
+        }
+        if (a.cu_nodes) {
+            const int n0 = max(a.cu_nodes[r], 0), nodes = min(min(a.cu_nodes[r + 1], a.rows) - n0, 32 * a.words);
+            for (int j = tid; j < nodes; j += 256)
+                if ((a.ancestors[(size_t)t * a.words + (j >> 5)] >> (j & 31)) & 1) {
+                    const int at = a.draft_tokens[n0 + j] - v0;
+                    if (at >= 0 && at < n) atomicAdd(&cnt[at], 1u);
+                }
+        }
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += 256) {
+        const bool allowed = !mask || ((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1);
+        const uint32_t c = counts ? cnt[i] : 0u;
+        if (!allowed) {
+            y[i] = -INFINITY;
+        } else if (c || !in_place) {
+            float v = x[i];
+            if (c) {
+                v = v > 0.f ? v / rep : v * rep;
+                const uint32_t k = c & ~ADJUST_SEEN;
+                if (k) v = v - freq * (float)k - pres;
+            }
+            y[i] = v;
+        }
+    }
+    if (a.cu_bias && has_request) {
+        // of equal tokens the last one listed counts: the largest place among them wins, by an integer maximum
+        const int b0 = min(max(a.cu_bias[r], 0), a.bias_len), b1 = min(max(a.cu_bias[r + 1], b0), a.bias_len);
+        if (b0 < b1) {
+            __syncthreads();
+            for (int i = b0 + tid; i < b1; i += 256) {
+                const int at = a.bias_ids[i] - v0;
+                if (at >= 0 && at < n) cnt[at] = 0;
+            }
+            __syncthreads();
+            for (int i = b0 + tid; i < b1; i += 256) {
+                const int at = a.bias_ids[i] - v0;
+                if (at >= 0 && at < n) atomicMax(&cnt[at], (uint32_t)(i - b0 + 1));
+            }
+            __syncthreads();
+            for (int i = b0 + tid; i < b1; i += 256) {
+                const int v = a.bias_ids[i], at = v - v0;
+                if (at >= 0 && at < n && cnt[at] == (uint32_t)(i - b0 + 1) && (!mask || ((mask[v >> 5] >> (v & 31)) & 1))) y[at] += a.bias_values[i];
+            }
+        }
+    }
+}
+
+TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, int requests, const int32_t* history, int history_len,
+                              const int32_t* cu_history, const int32_t* prompt_lens, const float* repetition, const float* presence,
+                              const float* frequency, const int32_t* bias_ids, const float* bias_values, int bias_len, const int32_t* cu_bias,
+                              const int32_t* masks, int num_masks, const int32_t* mask_rows, const int32_t* draft_tokens,
+                              const int32_t* cu_nodes, const int32_t* ancestors, int words, tff_stream_t stream) {
+    TFF_REQUIRE(rows >= 0 && V > 0 && requests >= 0, "adjust_logits: bad sizes rows=%d V=%d requests=%d", rows, V, requests);
+    if (rows == 0) return 0;
+    TFF_REQUIRE(logits && out && cu_history && prompt_lens && repetition && presence && frequency, "adjust_logits: null pointer");
+    TFF_REQUIRE(history_len >= 0 && (history || history_len == 0), "adjust_logits: a history of %d tokens without its tokens", history_len);
+    TFF_REQUIRE(bias_len >= 0 && (!cu_bias || bias_len == 0 || (bias_ids && bias_values)), "adjust_logits: %d biases without tokens and values",
+                bias_len);
+    TFF_REQUIRE(!mask_rows || num_masks == 0 || masks, "adjust_logits: rows with masks, and no masks");
+    TFF_REQUIRE(!cu_nodes || (draft_tokens && ancestors && words > 0), "adjust_logits: nodes without their tokens and ancestors");
+    TFF_REQUIRE(cu_nodes || rows == requests, "adjust_logits: %d rows of %d requests", rows, requests);
+    const int run = 8192, runs = (V + run - 1) / run;
+    TFF_REQUIRE((int64_t)rows * runs <= 0x7fffffff, "adjust_logits: %d rows of %d logits are more than a launch takes", rows, V);
+    const AdjustArgs a{logits, out, rows, V, runs, history, cu_history, prompt_lens, history_len, requests, repetition, presence, frequency,
+                       bias_ids, bias_values, cu_bias, bias_len, masks, masks ? num_masks : 0, (V + 31) / 32, mask_rows, draft_tokens, cu_nodes, ancestors, words};
+    adjust_logits_kernel<8192><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a);
+    return tff_check_launch("adjust_logits");
+}

@@ -587,6 +587,45 @@ TFF_API int tff_repetition_penalty(float* logits, int rows, int V, const int32_t
                                    const int32_t* cu_seen, const float* penalty,
                                    tff_stream_t stream);
 
+// ---- trees of drafted tokens (tree_attention.hip, draft_tree.hip) ----
+// A step brings R requests' trees: rows cu_nodes[r] .. cu_nodes[r + 1] - 1 are request r's nodes, node 0 the last token it has, a node's
+// parent before it.  ancestors [rows, words]: bit j of a row's words (32 a word, lowest first) says that it sees node j of its request: its
+// ancestors, and itself.  At most 32 words nodes a request, words at most 8.
+// Attention: node j's key and value lie in the request's pages at place start_pos[r] + j (tff_qk_norm_rope_kv puts them there); a node sees
+// the start_pos[r] cached places and the nodes of its bits, under a window the last `window` of them in this order.  A node
+// that sees nothing gets zeros, rows from cu_nodes[R] on are left as they are.  Head sizes up to 512.  out [rows, nq * d].
+TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const void* k_cache, const void* v_cache, const int32_t* block_tables,
+                               int bt_stride, const int32_t* cu_nodes, const int32_t* start_pos, const int32_t* ancestors, int words, int R,
+                               int rows, int nq, int nkv, int d, int page_size, int num_pages, int window, float scale, const float* sinks,
+                               float softcap, int dtype, tff_stream_t stream);
+// Which nodes are right: node 0, and after each the first of its children whose token (tokens [T]) is what the model chose after it
+// (choices [T]).  path [R, max_path]: the kept nodes, then -1; counts [R]; next [R]: the choice after the last of them.  A request
+// without nodes: 0 and -1.  A path of max_path nodes goes no further.
+TFF_API int tff_tree_accept(const int32_t* choices, const int32_t* tokens, const int32_t* cu_nodes, const int32_t* ancestors, int words, int T,
+                            int R, int max_path, int32_t* path, int32_t* counts, int32_t* next, tff_stream_t stream);
+// The kept nodes' keys and values to the places that follow the cached ones: for i < counts[r] what lies at place start_pos[r] + path[r, i]
+// goes to place start_pos[r] + i, in each of num_caches caches (layers) of one shape; the tables of pointers are on the host.  Any path
+// is right (all is read before any of it is written); a negative number, or a place outside the request's table, is passed over.  Two
+// requests must not share the pages of their nodes.  max_path at most 256.
+TFF_API int tff_cache_keep(void* const* k_caches, void* const* v_caches, int num_caches, const int32_t* block_tables, int bt_stride,
+                           const int32_t* start_pos, const int32_t* path, const int32_t* counts, int R, int max_path, int nkv, int d,
+                           int page_size, int num_pages, int dtype, tff_stream_t stream);
+
+// ---- options on logits (adjust_logits.hip) ----
+// Row t of logits [rows, V] to row t of out (the same tensor, or another): with the request's history (its prompt's prompt_lens[r] tokens, then
+// its output; tokens history[cu_history[r]] .. as they come, repeated ones and all)
+//   x / repetition[r] or, where x <= 0, x * repetition[r] for every token of the history; then - frequency[r] * n - presence[r] for
+//   every token that stands n > 0 times in its output; then + the value of the tokens bias_ids[cu_bias[r]] .. (of equal ones the last; cu_bias may
+//   be null); then -inf where the row's mask lacks the token's bit: row mask_rows[t] of masks [num_masks, ceil(V / 32)], none
+//   where mask_rows[t] is no row of it (mask_rows may be null).
+// Row t is request t's, or with cu_nodes a node of a tree (above): its request's, with the tokens (draft_tokens [rows]) of the nodes
+// it sees as further output; rows from cu_nodes[requests] on are copied.  Token ids outside the vocabulary are passed over.
+TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, int requests, const int32_t* history, int history_len,
+                              const int32_t* cu_history, const int32_t* prompt_lens, const float* repetition, const float* presence,
+                              const float* frequency, const int32_t* bias_ids, const float* bias_values, int bias_len, const int32_t* cu_bias,
+                              const int32_t* masks, int num_masks, const int32_t* mask_rows, const int32_t* draft_tokens,
+                              const int32_t* cu_nodes, const int32_t* ancestors, int words, tff_stream_t stream);
+
 // Draw from softmax(logits / temperature) restricted by top_k (0: off), top_p
 // (1: off) and min_p (0: off), by inverse CDF in index order with the given
 // uniform number per row.  temperature[r] <= 0 selects the argmax.  Probabilities

@@ -2603,6 +2603,203 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tenso
     return (out, probs) if return_probs else out
 
 
+# ---- options on logits, trees of drafted tokens ----
+
+def _int_row(t, name: str, n: int | None = None) -> int:
+    """The address of an int32 tensor of one dimension, of n elements where n is given."""
+    _req(t, name, torch.int32, 1)
+    if n is not None and t.numel() != n:
+        raise _lib.KernelError(f"{name}: {t.numel()} elements, expected {n}")
+    return t.data_ptr()
+
+
+def _one_device(what: str, device, *tensors) -> None:
+    """Operands on one device, which is the current one: a launch goes to the current device's stream."""
+    if device.index != torch.cuda.current_device():
+        raise _lib.KernelError(f"{what}: the operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise _lib.KernelError(f"{what}: operands on {device} and on {t.device}")
+
+
+#: words of 32 bits that a row of a tree's ancestors has at most
+TREE_WORDS = 8
+#: nodes that a path of kept nodes has at most
+TREE_PATH = 32 * TREE_WORDS
+
+
+def _ancestors(t, what: str, rows: int) -> int:
+    _req(t, what + " ancestors", torch.int32, 2)
+    if t.shape[0] != rows or not 0 < t.shape[1] <= TREE_WORDS:
+        raise _lib.KernelError(f"{what}: ancestors {tuple(t.shape)} are not [{rows}, 1 .. {TREE_WORDS}]")
+    return t.shape[1]
+
+
+def adjust_logits(logits: torch.Tensor, history: torch.Tensor, cu_history: torch.Tensor, prompt_lens: torch.Tensor,
+                  repetition: torch.Tensor, presence: torch.Tensor, frequency: torch.Tensor, bias=None, masks=None, drafts=None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """float32 logits [rows, V] after the requests' options, in a new tensor or in ``out`` (which may be ``logits``: then what no
+    option touches is neither read nor written).  Request r has the tokens ``history[cu_history[r]:cu_history[r + 1]]`` (int32, repeated
+    ones and all), of which the first ``prompt_lens[r]`` are its prompt and the rest its output, and float32 ``repetition`` (1: none),
+    ``presence`` and ``frequency`` (0: none) per request: logits of tokens in the history are divided by the first where positive and
+    multiplied elsewhere, those of tokens n > 0 times in the output get - frequency n - presence.  ``bias`` = (int32 ids, float32 values,
+    int32 cu [requests + 1]): numbers added to single tokens (of equal ones the last).  ``masks`` = (int32 [M, ceil(V / 32)],
+    int32 [rows]): the tokens a row may choose, a bit each (lowest first), and the row's mask (-1: none); the others get -inf.
+    ``drafts`` = (int32 tokens [rows], int32 cu_nodes [requests + 1], int32 ancestors [rows, words]): the rows are nodes of drafted trees
+    (:func:`tree_attention`) and have the tokens of the nodes they see as output, too; without it row i is request i's."""
+    _req(logits, "adjust_logits logits", torch.float32, 2)
+    rows, V = logits.shape
+    requests = cu_history.numel() - 1
+    if requests < 0:
+        raise _lib.KernelError("adjust_logits: cu_history has no elements")
+    _int_row(history, "adjust_logits history")
+    _int_row(cu_history, "adjust_logits cu_history")
+    _int_row(prompt_lens, "adjust_logits prompt_lens", requests)
+    for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
+        _req(t, name, torch.float32, 1)
+        if t.numel() != requests:
+            raise _lib.KernelError(f"adjust_logits: {t.numel()} numbers of {name} for {requests} requests")
+    ids = values = cu_bias = mask_bits = mask_rows = tokens = cu_nodes = ancestors = None
+    words = 0
+    if bias is not None:
+        ids, values, cu_bias = bias
+        _int_row(ids, "adjust_logits bias ids")
+        _int_row(cu_bias, "adjust_logits cu_bias", requests + 1)
+        _req(values, "adjust_logits bias values", torch.float32, 1)
+        if values.numel() != ids.numel():
+            raise _lib.KernelError(f"adjust_logits: {values.numel()} biases for {ids.numel()} tokens")
+    if masks is not None:
+        mask_bits, mask_rows = masks
+        _req(mask_bits, "adjust_logits masks", torch.int32, 2)
+        if mask_bits.shape[1] != -(-V // 32):
+            raise _lib.KernelError(f"adjust_logits: masks of {mask_bits.shape[1]} words for {V} tokens")
+        _int_row(mask_rows, "adjust_logits mask rows", rows)
+    if drafts is not None:
+        tokens, cu_nodes, ancestors = drafts
+        _int_row(tokens, "adjust_logits draft tokens", rows)
+        _int_row(cu_nodes, "adjust_logits cu_nodes", requests + 1)
+        words = _ancestors(ancestors, "adjust_logits", rows)
+    elif rows != requests:
+        raise _lib.KernelError(f"adjust_logits: {rows} rows of {requests} requests")
+    if out is None:
+        out = torch.empty_like(logits)
+    elif out is not logits:
+        _req(out, "adjust_logits out", torch.float32, 2)
+        if out.shape != logits.shape:
+            raise _lib.KernelError(f"adjust_logits out: shape {tuple(out.shape)} is not {(rows, V)}")
+        if out.data_ptr() != logits.data_ptr() and abs(out.data_ptr() - logits.data_ptr()) < 4 * rows * V:
+            raise _lib.KernelError("adjust_logits out: overlaps the logits without being them")
+    _one_device("adjust_logits", logits.device, history, cu_history, prompt_lens, repetition, presence, frequency, ids, values, cu_bias,
+                mask_bits, mask_rows, tokens, cu_nodes, ancestors, out)
+    _lib.check(_lib.load().tff_adjust_logits(
+        logits.data_ptr(), out.data_ptr(), rows, V, requests, history.data_ptr(), history.numel(), cu_history.data_ptr(),
+        prompt_lens.data_ptr(), repetition.data_ptr(), presence.data_ptr(), frequency.data_ptr(), _ptr(ids), _ptr(values),
+        0 if ids is None else ids.numel(), _ptr(cu_bias), _ptr(mask_bits), 0 if mask_bits is None else mask_bits.shape[0], _ptr(mask_rows),
+        _ptr(tokens), _ptr(cu_nodes), _ptr(ancestors), words, _stream()))
+    return out
+
+
+def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_tables: torch.Tensor, cu_nodes: torch.Tensor, start_pos: torch.Tensor, ancestors: torch.Tensor, window: int = 0,
+                   scale: float | None = None, sinks: torch.Tensor | None = None, softcap: float = 0.0,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of trees of drafted tokens: rows ``cu_nodes[r]:cu_nodes[r + 1]`` of ``q`` [rows, >= nq * d] are request r's nodes, whose
+    keys and values lie in its pages from place ``start_pos[r]`` on (as :func:`qk_norm_rope_kv` puts them there, at positions by their
+    depth).  A node sees the places before and the nodes whose bit its row of ``ancestors`` (int32 [rows, words], 32 nodes a word,
+    lowest bit first, its own among them) has; under a ``window`` the last so many of these.  ``sinks`` (float32 [nq]) and ``softcap``:
+    see :func:`paged_attention`.  Returns [rows, nq * d] in q's type, which is the cache's; a node that sees nothing gets zeros, rows that
+    no request has are left as they are.  Up to 256 nodes a request, head sizes up to 512; a token's bits may depend on what else is in the
+    step, as they do where decoding splits keys.  The table of pages has to reach to a request's last node."""
+    _req(q, "tree_attention q", ndim=2)
+    rows = q.shape[0]
+    if q.shape[1] < nq * d:
+        raise _lib.KernelError(f"tree_attention q: rows of {q.shape[1]} hold fewer than nq*d = {nq * d}")
+    _req(k_cache, "k cache", q.dtype, 4)
+    _req(v_cache, "v cache", q.dtype, 4)
+    _check_cache(k_cache, v_cache, nkv, d, "tree_attention")
+    _req(block_tables, "block tables", torch.int32, 2)
+    R = start_pos.numel()
+    _int_row(start_pos, "tree_attention start_pos")
+    _int_row(cu_nodes, "tree_attention cu_nodes", R + 1)
+    if block_tables.shape[0] != R:
+        raise _lib.KernelError(f"tree_attention: tables of {block_tables.shape[0]} requests for {R}")
+    words = _ancestors(ancestors, "tree_attention", rows)
+    _check_sinks(sinks, nq)
+    if out is None:
+        out = torch.empty(rows, nq * d, dtype=q.dtype, device=q.device)
+    else:
+        _req(out, "tree_attention out", q.dtype, 2)
+        if tuple(out.shape) != (rows, nq * d):
+            raise _lib.KernelError(f"tree_attention out: shape {tuple(out.shape)} is not {(rows, nq * d)}")
+    _one_device("tree_attention", q.device, k_cache, v_cache, block_tables, cu_nodes, start_pos, ancestors, sinks, out)
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    _lib.check(_lib.load().tff_tree_attention(
+        q.data_ptr(), q.stride(0), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+        block_tables.stride(0), cu_nodes.data_ptr(), start_pos.data_ptr(), ancestors.data_ptr(), words, R, rows, nq, nkv, d,
+        k_cache.shape[2], k_cache.shape[0], int(window), float(scale), _ptr(sinks), float(softcap or 0.0), dtype_code(q.dtype), _stream()))
+    return out
+
+
+def tree_accept(choices: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Tensor, ancestors: torch.Tensor, max_path: int):
+    """Which nodes of drafted trees (:func:`tree_attention`) are right: from node 0 on, which the request already has, the first child
+    whose token is what the model chose after its parent (``choices``, ``tokens``: int32 [rows]).  Returns int32 ``path``
+    [requests, max_path] (the kept nodes' numbers in their tree, then -1), ``counts`` [requests] and ``next`` [requests], the choice after
+    the last kept node; a request without nodes gets 0 and -1.  A path ends at ``max_path`` nodes."""
+    T, R = tokens.numel(), cu_nodes.numel() - 1
+    _int_row(tokens, "tree_accept tokens")
+    _int_row(choices, "tree_accept choices", T)
+    _int_row(cu_nodes, "tree_accept cu_nodes")
+    if R < 0:
+        raise _lib.KernelError("tree_accept: cu_nodes has no elements")
+    words = _ancestors(ancestors, "tree_accept", T)
+    if not 0 < max_path <= TREE_PATH:
+        raise _lib.KernelError(f"tree_accept: paths of {max_path} nodes (1 .. {TREE_PATH})")
+    _one_device("tree_accept", tokens.device, choices, cu_nodes, ancestors)
+    made = torch.empty(R * (max_path + 2), dtype=torch.int32, device=tokens.device)
+    path, counts, following = made[:R * max_path].view(R, max_path), made[R * max_path:R * (max_path + 1)], made[R * (max_path + 1):]
+    _lib.check(_lib.load().tff_tree_accept(choices.data_ptr(), tokens.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, T, R,
+                                           int(max_path), path.data_ptr(), counts.data_ptr(), following.data_ptr(), _stream()))
+    return path, counts, following
+
+
+def cache_keep(caches: list, block_tables: torch.Tensor, start_pos: torch.Tensor, path: torch.Tensor, counts: torch.Tensor) -> None:
+    """Moves the keys and values of the kept nodes to the places that follow the cached ones, in place and in all ``caches`` (a list of
+    (keys, values) of one shape, as the layers of a group have them) at once: for i < counts[r], place ``start_pos[r] + path[r, i]`` of
+    request r's pages to place ``start_pos[r] + i``.  ``path`` int32 [requests, up to 256] and ``counts`` as :func:`tree_accept` returns
+    them.  Two requests must not share the pages that their nodes lie in."""
+    R = start_pos.numel()
+    _int_row(start_pos, "cache_keep start_pos")
+    _int_row(counts, "cache_keep counts", R)
+    _req(path, "cache_keep path", torch.int32, 2)
+    _req(block_tables, "block tables", torch.int32, 2)
+    if path.shape[0] != R or block_tables.shape[0] != R or not 0 < path.shape[1] <= TREE_PATH:
+        raise _lib.KernelError(f"cache_keep: paths {tuple(path.shape)} and tables {tuple(block_tables.shape)} for {R} requests")
+    if not caches:
+        return
+    shape, dtype, device = caches[0][0].shape, caches[0][0].dtype, caches[0][0].device
+    if len(shape) != 4:
+        raise _lib.KernelError(f"k cache: expected 4 dimensions, got shape {tuple(shape)}")
+    pages, nkv, page_size, d = shape
+    vshape, keys, values = (pages, nkv, d, page_size), [], []
+    for k, v in caches:
+        if k.shape != shape or v.shape != vshape or k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device \
+                or not k.is_contiguous() or not v.is_contiguous():
+            raise _lib.KernelError(f"cache_keep: caches {tuple(k.shape)} / {tuple(v.shape)} of {k.dtype} beside {tuple(shape)} of {dtype}")
+        keys.append(k.data_ptr())
+        values.append(v.data_ptr())
+    if not caches[0][0].is_cuda:
+        raise _lib.KernelError("cache_keep: expected a tensor on the GPU")
+    _one_device("cache_keep", device, block_tables, start_pos, path, counts)
+    n = len(keys)
+    if len(set(keys)) != n or len(set(values)) != n:
+        raise _lib.KernelError("cache_keep: a cache is listed twice")
+    kp, vp = (ctypes.c_void_p * n)(*keys), (ctypes.c_void_p * n)(*values)
+    _lib.check(_lib.load().tff_cache_keep(
+        ctypes.addressof(kp), ctypes.addressof(vp), n, block_tables.data_ptr(), block_tables.stride(0), start_pos.data_ptr(), path.data_ptr(),
+        counts.data_ptr(), R, path.shape[1], nkv, d, page_size, pages, dtype_code(dtype), _stream()))
+
+
 def measure_ceilings(device="cuda:0", gib: float = 4.0, quick: bool = False) -> dict:
     """What this machine gives to kernels that do nothing else: streaming reads
     from HBM into registers (a buffer of ``gib`` GiB, far larger than the
@@ -2683,5 +2880,9 @@ OP_TABLE = {
     "cast": cast,
     "argmax": argmax,
     "repetition_penalty": repetition_penalty,
+    "adjust_logits": adjust_logits,
+    "tree_attention": tree_attention,
+    "tree_accept": tree_accept,
+    "cache_keep": cache_keep,
     "sample": sample,
 }
