@@ -16,7 +16,7 @@ def _refused(name, args, what):
 
 
 ATTENTION = dict(q=P, q_stride=256, out=P, k=P, v=P, bt=P, bt_stride=4, cu=P, start=P, anc=P, words=1, R=1, rows=3, nq=4, nkv=2, d=64, page=16,
-                 pages=8, window=0, scale=0.125, sinks=None, softcap=0.0, dtype=1, stream=None)
+                 pages=8, window=0, scale=0.125, sinks=None, softcap=0.0, ws=None, ws_bytes=0, dtype=1, stream=None)
 
 
 @pytest.mark.parametrize("change, what", [

@@ -597,7 +597,10 @@ TFF_API int tff_repetition_penalty(float* logits, int rows, int V, const int32_t
 TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const void* k_cache, const void* v_cache, const int32_t* block_tables,
                                int bt_stride, const int32_t* cu_nodes, const int32_t* start_pos, const int32_t* ancestors, int words, int R,
                                int rows, int nq, int nkv, int d, int page_size, int num_pages, int window, float scale, const float* sinks,
-                               float softcap, int dtype, tff_stream_t stream);
+                               float softcap, void* workspace, size_t workspace_bytes, int dtype, tff_stream_t stream);
+// Device memory, 16-byte aligned, for the partial results of keys that several blocks share (0: these sizes need none, and run on the
+// general kernel, as a call without it does).
+TFF_API size_t tff_tree_attention_workspace_bytes(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype);
 // Which nodes are right: node 0, and after each the first of its children whose token (tokens [T]) is what the model chose after it
 // (choices [T]).  path [R, max_path]: the kept nodes, then -1; counts [R]; next [R]: the choice after the last of them.  A request
 // without nodes: 0 and -1.  A path of max_path nodes goes no further.

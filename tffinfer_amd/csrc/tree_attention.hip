@@ -5,6 +5,7 @@
 // over the visible places j; under a window of w only the last w of them in the order of their places.  A node that sees nothing gets zeros.
 // The reference has one row of a causal mask per token (src/kernel/cuda/mask_op.cu:37-43) and no trees.
 #include "common.h"
+#include "mfma_tiles.h"
 #include "tffinfer_kernels.h"
 
 #define TREE_WORDS 8                 // words of 32 bits a row of ancestors has at most: 256 nodes
@@ -30,20 +31,24 @@ __device__ __forceinline__ TreeRow tree_row(const int32_t* __restrict__ row, int
     int count = 0;
 #pragma unroll
     for (int w = 0; w < TREE_WORDS; ++w) {
-        const int left = nodes - 32 * w;
-        t.bits[w] = w < words && left > 0 ? (uint32_t)row[w] & (left >= 32 ? ~0u : (1u << left) - 1) : 0u;
+        const int left = w < words ? nodes - 32 * w : 0;
+        t.bits[w] = (uint32_t)row[min(w, words - 1)] & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u);
         count += __popc(t.bits[w]);
     }
     t.lo = 0;
     if (window > 0) {
         t.lo = max(0, min(start, start + count - window));
-        int drop = count - window;           // the window ends among the nodes
+        for (int drop = count - window; drop > 0; --drop) {      // (the window ends among the nodes)
+            bool done = false;
 #pragma unroll
-        for (int w = 0; w < TREE_WORDS; ++w)
-            while (drop > 0 && t.bits[w]) {
-                t.bits[w] &= t.bits[w] - 1;
-                --drop;
+            for (int w = 0; w < TREE_WORDS; ++w) {
+                const uint32_t x = t.bits[w];
+                if (!done && x) {
+                    t.bits[w] = x & (x - 1);
+                    done = true;
+                }
             }
+        }
     }
     return t;
 }
@@ -131,10 +136,570 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
     }
 }
 
+// ---- on the matrix cores: bfloat16 and float32, head sizes 64, 128 and 256, pages of a power of two of tokens, at least 8 ----
+// The columns of a request and kv head are its (node, q head of the group) pairs, node * G + head, in groups of 16 CT.  The work
+// is cut into units of one slice of keys (32 in bfloat16, 16 in float32) and one group of columns; every block finds out by itself, from the
+// requests' tables, which run of units is its own (total / blocks of them, consecutive: the slices of a group of columns, then the next
+// group's, then the next request's), so that blocks end together whatever the requests' lengths, nothing is planned on the host and a
+// captured launch serves any lengths.  The four waves of a block take every fourth slice, with all the block's columns in
+// registers: a key or value goes from memory into the registers of one wave and into no other, no LDS and no barrier in the loop.  S^T = K Q^T
+// and O^T = V^T P^T: a lane's scores, weights and outputs all belong to column lane % 16, and with the keys in the order below the
+// scores' registers are the second product's operand as they lie.  The maximum that the exponentials are taken against follows the true one
+// when that is more than 2^8 ahead: the outputs are rescaled some times a run, not at every slice.  At a run's end the four waves meet in LDS; a
+// group of columns whose slices went to several blocks leaves a partial result with each, merged by a second kernel.
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 tree_bf16x8;
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float tree_f32x4;
+typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t tree_u32x4;
+
+#define TREE_LAG 8.0f                // log2 of what the running maximum may be behind
+
+template <typename T, int D>
+struct TreeMath;
+template <int D>
+struct TreeMath<bf16_t, D> {
+    static constexpr int SLICE = 32, TILES = 2, PER = 8;     // keys of a slice, score tiles, elements of a 16-byte load
+    static constexpr int QF = D / 32, KF = 2 * QF, VF = D / 16;
+    typedef tree_bf16x8 frag;
+    // scores of tile t (rows 4 kg + e: keys 8 kg + 4 t + e of the slice)
+    static __device__ __forceinline__ tree_f32x4 scores(const frag (&k)[KF], const frag (&q)[QF], int t) {
+        tree_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < QF; ++f) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t * QF + f], q[f], s, 0, 0, 0);
+        return s;
+    }
+    static __device__ __forceinline__ void add(tree_f32x4 (&o)[D / 16], const frag (&v)[VF], const float (&p)[4 * TILES]) {
+        frag w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = (bf16_t)p[i];       // (a weight rounds to bfloat16, half a step of 2^-8, as the product takes it)
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[dt], w, o[dt], 0, 0, 0);
+    }
+    // where a lane's row of key fragment f lies: (key of the slice, element)
+    static __device__ __forceinline__ int key_row(int f, int qc) { return 8 * (qc >> 2) + 4 * (f / QF) + (qc & 3); }
+    static __device__ __forceinline__ int key_elem(int f, int kg) { return (f % QF) * 32 + kg * 8; }
+    static __device__ __forceinline__ int key_block(int qc) { return qc >> 2; }      // the eight keys it is among
+    static __device__ __forceinline__ int value_key(int kg) { return 8 * kg; }       // first key of a lane's values
+    // Zeros in the elements whose bit `live` has not; the bits of those left that are not finite come back.
+    static __device__ __forceinline__ uint32_t clean(frag (&v)[VF], uint32_t live) {
+        uint32_t keep[4], bad[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            keep[w] = ((live >> (2 * w)) & 1 ? 0xffffu : 0u) | ((live >> (2 * w + 1)) & 1 ? 0xffff0000u : 0u);
+            bad[w] = 0;
+        }
+#pragma unroll
+        for (int dt = 0; dt < VF; ++dt) {
+            tree_u32x4 x = __builtin_bit_cast(tree_u32x4, v[dt]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                x[w] &= keep[w];
+                bad[w] |= (x[w] & 0x7f807f80u) + 0x00800080u;        // (bit 15 of a half: its exponent is all ones)
+            }
+            v[dt] = __builtin_bit_cast(frag, x);
+        }
+        uint32_t odd = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) odd |= (((bad[w] >> 15) & 1) | ((bad[w] >> 30) & 2)) << (2 * w);
+        return odd;
+    }
+    static __device__ __forceinline__ void only_finite(frag (&v)[VF]) {
+#pragma unroll
+        for (int dt = 0; dt < VF; ++dt) {
+            tree_u32x4 x = __builtin_bit_cast(tree_u32x4, v[dt]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if ((x[w] & 0x7f80u) == 0x7f80u) x[w] &= 0xffff0000u;
+                if ((x[w] & 0x7f800000u) == 0x7f800000u) x[w] &= 0xffffu;
+            }
+            v[dt] = __builtin_bit_cast(frag, x);
+            __builtin_amdgcn_sched_barrier(0);                       // (one after the other: no registers for all of them)
+        }
+    }
+};
+template <int D>
+struct TreeMath<float, D> {
+    static constexpr int SLICE = 16, TILES = 1, PER = 4;
+    static constexpr int QF = D / 16, KF = QF, VF = D / 16;
+    typedef tree_f32x4 frag;
+    static __device__ __forceinline__ tree_f32x4 scores(const frag (&k)[KF], const frag (&q)[QF], int) {
+        tree_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < QF; ++f)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[f][e], q[f][e], s, 0, 0, 0);
+        return s;
+    }
+    static __device__ __forceinline__ void add(tree_f32x4 (&o)[D / 16], const frag (&v)[VF], const float (&p)[4 * TILES]) {
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[dt][e], p[e], o[dt], 0, 0, 0);
+    }
+    static __device__ __forceinline__ int key_row(int, int qc) { return qc; }
+    static __device__ __forceinline__ int key_elem(int f, int kg) { return f * 16 + kg * 4; }
+    static __device__ __forceinline__ int key_block(int qc) { return qc >> 3; }
+    static __device__ __forceinline__ int value_key(int kg) { return 4 * kg; }
+    static __device__ __forceinline__ uint32_t clean(frag (&v)[VF], uint32_t live) {
+        bool bad[4] = {false, false, false, false};
+#pragma unroll
+        for (int dt = 0; dt < VF; ++dt)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                if (!((live >> w) & 1)) v[dt][w] = 0.f;
+                bad[w] |= !(fabsf(v[dt][w]) < INFINITY);
+            }
+        return (bad[0] ? 1u : 0u) | (bad[1] ? 2u : 0u) | (bad[2] ? 4u : 0u) | (bad[3] ? 8u : 0u);
+    }
+    static __device__ __forceinline__ void only_finite(frag (&v)[VF]) {
+#pragma unroll
+        for (int dt = 0; dt < VF; ++dt)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v[dt][w] = fabsf(v[dt][w]) < INFINITY ? v[dt][w] : 0.f;
+    }
+};
+
+struct TreeArgs {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int32_t *block_tables, *cu_nodes, *start_pos, *ancestors;
+    const float* sinks;
+    float *part_o, *part_ml;         // [kv head][block][2][columns][D], [..][columns][2]
+    int q_stride, bt_stride, words, R, rows, nq, nkv, page_size, page_shift, num_pages, window, blocks;
+    float scale, softcap;
+};
+
+// One request's share of the work.
+struct TreeRequest {
+    int n0, nodes, start, end, first;    // its first row, nodes, cached places, places, and the first place that a slice begins with
+    int slices, groups;
+};
+template <int SLICE, int COLS>
+__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
+    TreeRequest t;
+    t.n0 = max(a.cu_nodes[r], 0);
+    t.nodes = max(0, min(min(a.cu_nodes[r + 1], a.rows) - t.n0, 32 * a.words));
+    const long long room = (long long)a.bt_stride * a.page_size;
+    t.start = (int)min((long long)max(a.start_pos[r], 0), room);
+    t.end = (int)min((long long)t.start + t.nodes, room);
+    t.first = a.window > 0 ? max(0, t.start - a.window) / 32 * 32 : 0;
+    t.groups = (t.nodes * (a.nq / a.nkv) + COLS - 1) / COLS;
+    // (a request with nodes has a slice even where its table has no room for them: its rows are written)
+    t.slices = t.nodes > 0 ? max(1, (t.end - t.first + SLICE - 1) / SLICE) : 0;
+    return t;
+}
+__device__ __forceinline__ int tree_wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v, o, 64);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+// Units of all requests, and of those before request `upto`; the same in every lane.
+template <int SLICE, int COLS>
+__device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& total, int& before) {
+    total = before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        int u = 0;
+        if (r < a.R) {
+            const TreeRequest t = tree_request<SLICE, COLS>(a, r);
+            u = t.slices * t.groups;
+        }
+        const int incl = tree_wave_scan(u);
+        if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
+}
+// How many units a block takes: an equal share, and no less than two slices a wave (a wave that has one waits for memory once and then for
+// the other waves).
+__device__ __forceinline__ int tree_share(int total, int blocks) { return max((total + blocks - 1) / blocks, 8); }
+
+template <typename T, int D, int CT, int OCC>
+__global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs a) {
+    typedef TreeMath<T, D> M;
+    typedef typename M::frag frag;
+    constexpr int COLS = 16 * CT, SLICE = M::SLICE, KEYS = 4 * M::TILES, LD = D + 4;
+    __shared__ __attribute__((aligned(16))) float merge_o[4 * COLS * LD];    // a wave's outputs, [column][D] (4 more: banks)
+    __shared__ float merge_m[4 * COLS], merge_l[4 * COLS];
+    __shared__ uint32_t see[COLS * (TREE_WORDS + 1)];                        // the columns' bits, and a word of zeros
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), qc = lane & 15, kg = lane >> 4;
+    const int g = blockIdx.x % a.nkv, b = blockIdx.x / a.nkv, G = a.nq / a.nkv;
+    const size_t page_stride = (size_t)a.nkv * a.page_size * D;
+    const T* __restrict__ kc = (const T*)a.k_cache + (size_t)g * a.page_size * D;
+    const T* __restrict__ vc = (const T*)a.v_cache + (size_t)g * a.page_size * D;
+    const float log2e = 1.4426950408889634f;
+
+    // the block's run of units, and the request that it begins in
+    int total, before;
+    tree_units<SLICE, COLS>(a, 0, total, before);
+    const int share = tree_share(total, a.blocks), u0 = min(total, b * share), u1 = min(total, u0 + share);
+    if (u0 >= u1) return;
+    int r = 0;
+    before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        const int rr = r0 + lane;
+        int u = 0;
+        if (rr < a.R) {
+            const TreeRequest t = tree_request<SLICE, COLS>(a, rr);
+            u = t.slices * t.groups;
+        }
+        const int incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
+        if (before + all <= u0) {
+            before += all;
+            continue;
+        }
+        const int at = __ffsll((long long)__ballot(before + incl > u0)) - 1;
+        r = r0 + at;
+        before += at > 0 ? __builtin_amdgcn_readlane(incl, at - 1) : 0;
+        break;
+    }
+
+    for (int u = u0; u < u1;) {
+        const TreeRequest t = tree_request<SLICE, COLS>(a, r);
+        const int mine = t.slices * t.groups;
+        if (u >= before + mine) {
+            before += mine;
+            ++r;
+            continue;
+        }
+        const int group = (u - before) / t.slices, s0 = u - before - group * t.slices;
+        const int s1 = min(t.slices, s0 + (u1 - u));
+        const int ncols = min(COLS, t.nodes * G - group * COLS);
+        const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
+
+        // the columns: queries, bits, the first cached place of each
+        frag q[CT][M::QF];
+        int lo[CT], lo_least = t.end, lo_most = 0;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            const int c = min(ct * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
+            const T* qp = (const T*)a.q + (size_t)(t.n0 + node) * a.q_stride + (size_t)head * D;
+#pragma unroll
+            for (int f = 0; f < M::QF; ++f) q[ct][f] = *reinterpret_cast<const frag*>(qp + M::key_elem(f, kg));
+            lo[ct] = 0;
+        }
+        __syncthreads();                 // (the run before is merged)
+        for (int c = tid; c < COLS; c += 256) {
+            const int node = (min(c, ncols - 1) + group * COLS) / G;
+            const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + node) * a.words, a.words, t.end - t.start, t.start, a.window);
+#pragma unroll
+            for (int w = 0; w < TREE_WORDS; ++w) see[c * (TREE_WORDS + 1) + w] = row.bits[w];
+            see[c * (TREE_WORDS + 1) + TREE_WORDS] = 0;
+            merge_m[c] = __int_as_float(row.lo);
+        }
+        __syncthreads();
+        if (a.window > 0) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                lo[ct] = __float_as_int(merge_m[ct * 16 + qc]);
+                lo_least = min(lo_least, lo[ct]);
+                lo_most = max(lo_most, lo[ct]);
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                lo_least = min(lo_least, __shfl_xor(lo_least, o, 64));
+                lo_most = max(lo_most, __shfl_xor(lo_most, o, 64));
+            }
+            lo_least = __builtin_amdgcn_readfirstlane(lo_least);
+            lo_most = __builtin_amdgcn_readfirstlane(lo_most);
+            __syncthreads();             // (merge_m is written at the run's end)
+        } else {
+            lo_least = 0;
+        }
+
+        tree_f32x4 o[CT][D / 16];
+        float m[CT], l[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            m[ct] = -INFINITY;
+            l[ct] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) o[ct][dt] = tree_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        // places of slice s that a lane loads from: pages two slices ahead, so that no load of a page number waits behind keys and values
+        const int last_block = (max(t.end, 1) - 1) >> 3;         // blocks of eight places lie in one page
+        auto place = [&](int s, int block) { return min(((t.first + s * SLICE) >> 3) + block, last_block) << 3; };
+        auto page_of = [&](int at) {
+            const int p = bt[at >> a.page_shift];
+            return (unsigned)p < (unsigned)a.num_pages ? p : 0;
+        };
+        auto slot_of = [&](int at) { return at & (a.page_size - 1); };
+        const int kb = M::key_block(qc), vb = M::value_key(kg) >> 3;
+        frag k[M::KF], v[M::VF];
+        auto load_k = [&](int s, int page) {
+            const int at = place(s, kb);
+            const T* p = kc + (size_t)page * page_stride + (size_t)slot_of(at) * D;
+#pragma unroll
+            for (int f = 0; f < M::KF; ++f) k[f] = *reinterpret_cast<const frag*>(p + (M::key_row(f, qc) & 7) * D + M::key_elem(f, kg));
+        };
+        auto load_v = [&](int s, int page) {
+            const int at = place(s, vb) + (M::value_key(kg) & 7);
+            const T* p = vc + (size_t)page * page_stride + slot_of(at) + (size_t)qc * a.page_size;
+#pragma unroll
+            for (int dt = 0; dt < M::VF; ++dt) {
+                v[dt] = *reinterpret_cast<const frag*>(p);
+                p += 16 * a.page_size;
+            }
+        };
+
+        // which of the places key, key + 1, ... column ct * 16 + qc sees: a bit each (the next 8 of them hold)
+        auto visible = [&](int ct, int key) {
+            const int j = key - t.start;
+            const uint32_t* row = see + (ct * 16 + qc) * (TREE_WORDS + 1);
+            if (j >= 0) {
+                const int w = min(j >> 5, TREE_WORDS - 1);
+                return j < 32 * TREE_WORDS ? __funnelshift_r(row[w], row[w + 1], j & 31) : 0u;
+            }
+            const int cached = min(-j, 31), below = min(max(lo[ct] - key, 0), 31);
+            return (((1u << cached) - 1) & (~0u << below)) | (-j < 32 ? row[0] << -j : 0u);
+        };
+
+        // A slice's keys are asked for as soon as the slice before is multiplied, its values as soon as that one's are: either is on its way while
+        // the wave works on the other, in one set of registers.
+        int s = s0 + wv, pk = 0, pv = 0;
+        if (s < s1) {
+            load_k(s, page_of(place(s, kb)));
+            load_v(s, page_of(place(s, vb)));
+            pk = page_of(place(s + 4, kb));
+            pv = page_of(place(s + 4, vb));
+        }
+        for (; s < s1; s += 4) {
+            const int k0 = t.first + s * SLICE;
+            const bool masked = k0 + SLICE > t.start || k0 < lo_most;
+            const int pk2 = page_of(place(s + 8, kb)), pv2 = page_of(place(s + 8, vb));
+            float p[CT][KEYS];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int tile = 0; tile < M::TILES; ++tile) {
+                    const tree_f32x4 sc = M::scores(k, q[ct], tile);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[ct][4 * tile + e] = sc[e];
+                }
+            if (s + 4 < s1) load_k(s + 4, pk);
+            if (a.softcap > 0.f) {
+                // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, as a score of its size is anyway
+                const float in = -2.f * a.scale / a.softcap * log2e, outer = a.softcap * log2e;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(-fabsf(p[ct][i] * in)), h = outer * (1.f - e) / (1.f + e);
+                        p[ct][i] = copysignf(h, p[ct][i] * a.scale);
+                    }
+            } else {
+                const float f = a.scale * log2e;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) p[ct][i] *= f;
+            }
+            if (masked) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    const uint32_t sees = visible(ct, k0 + M::value_key(kg));
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i)
+                        if (!((sees >> i) & 1)) p[ct][i] = -INFINITY;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                float top = p[ct][0];
+#pragma unroll
+                for (int i = 1; i < KEYS; ++i) top = fmaxf(top, p[ct][i]);
+                top = rows_max(top);
+                const bool ahead = top > m[ct] + TREE_LAG;
+                if (__any(ahead)) {
+                    const float now = ahead ? top : m[ct], f = ahead ? __builtin_amdgcn_exp2f(m[ct] - now) : 1.f;
+                    m[ct] = now;
+                    l[ct] *= f;
+#pragma unroll
+                    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[ct][dt][e] *= f;
+                }
+                const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    p[ct][i] = __builtin_amdgcn_exp2f(p[ct][i] - ref);
+                    l[ct] += p[ct][i];
+                }
+            }
+            if (masked) {
+                // Values of places that no column sees: what lies there is anything.  And a value that is not finite may only reach the columns that
+                // see it: zero times it would not be zero.  The product takes zeros in their places, and who sees one has it added.
+                uint32_t live = 0;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) {
+                    const int key = k0 + M::value_key(kg) + i;
+                    if (key < t.end && key >= lo_least) live |= 1u << i;
+                }
+                uint32_t odd = M::clean(v, live) << M::value_key(kg);
+                if (__any(odd != 0)) {
+                    M::only_finite(v);
+#pragma unroll
+                    for (int x = 1; x < 64; x <<= 1) odd |= (uint32_t)__shfl_xor((int)odd, x, 64);
+                    for (uint32_t left = __builtin_amdgcn_readfirstlane(odd); left; left &= left - 1) {
+                        const int key = k0 + __ffs((int)left) - 1;
+                        const T* vp = vc + (size_t)page_of(key) * page_stride + slot_of(key) + (size_t)(4 * kg) * a.page_size;
+                        uint32_t sees[CT];
+#pragma unroll
+                        for (int ct = 0; ct < CT; ++ct) sees[ct] = visible(ct, key);
+#pragma unroll
+                        for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float x = to_f32(*vp);
+                                vp += e < 3 ? a.page_size : 13 * a.page_size;
+#pragma unroll
+                                for (int ct = 0; ct < CT; ++ct)
+                                    if ((sees[ct] & 1) && !(fabsf(x) < INFINITY)) o[ct][dt][e] += x;
+                                asm volatile("" ::: "memory");       // (one element after the other: no registers for all of them)
+                            }
+                    }
+                }
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) M::add(o[ct], v, p[ct]);
+            if (s + 4 < s1) load_v(s + 4, pv);
+            pk = pk2;
+            pv = pv2;
+        }
+
+        // the four waves' results together (addresses from a lane number taken here: not kept in registers through the loop)
+        const int lane2 = w4_lane(), qc2 = lane2 & 15, kg2 = lane2 >> 4, tid2 = wv * 64 + lane2;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            const float sum = rows_sum(l[ct]);
+            if (kg2 == 0) {
+                merge_m[wv * COLS + ct * 16 + qc2] = m[ct];
+                merge_l[wv * COLS + ct * 16 + qc2] = sum;
+            }
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt)
+                *reinterpret_cast<tree_f32x4*>(&merge_o[(wv * COLS + ct * 16 + qc2) * LD + dt * 16 + 4 * kg2]) = o[ct][dt];
+        }
+        __syncthreads();
+        const bool whole = s0 == 0 && s1 == t.slices;
+        const size_t part = (((size_t)g * a.blocks + b) * 2 + (u == u0 ? 0 : 1)) * COLS;
+        for (int i = tid2; i < ncols * (D / 4); i += 256) {
+            const int c = i / (D / 4), e = (i - c * (D / 4)) * 4;
+            float top = merge_m[c];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = fmaxf(top, merge_m[w * COLS + c]);
+            const float ref = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
+            tree_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(merge_m[w * COLS + c] - ref);
+                const tree_f32x4 ow = *reinterpret_cast<const tree_f32x4*>(&merge_o[(w * COLS + c) * LD + e]);
+                sum += merge_l[w * COLS + c] * f;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) acc[z] += ow[z] * f;
+            }
+            if (whole) {
+                const int cc = c + group * COLS, node = cc / G, head = g * G + (cc - node * G);
+                if (a.sinks) {
+                    const float sink = a.sinks[head] * log2e;
+                    if (top == -INFINITY) sum = 1.f;         // (nothing seen: zeros)
+                    else sum += __builtin_amdgcn_exp2f(sink - top);
+                }
+                const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
+                T* op = (T*)a.out + ((size_t)(t.n0 + node) * a.nq + head) * D + e;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) op[z] = from_f32<T>(acc[z] * inv);
+            } else {
+                *reinterpret_cast<tree_f32x4*>(a.part_o + (part + c) * D + e) = acc;
+                if (e == 0) {
+                    a.part_ml[(part + c) * 2] = top;
+                    a.part_ml[(part + c) * 2 + 1] = sum;
+                }
+            }
+        }
+        u += s1 - s0;
+    }
+}
+
+// The partial results of a group of columns, in the order of the keys: a block a node, a wave a q head after the other.
+template <typename T, int D, int CT>
+__global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
+    constexpr int COLS = 16 * CT, SLICE = TreeMath<T, D>::SLICE, N = D / 64;
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, G = a.nq / a.nkv;
+    const int r = tree_row_request(a.cu_nodes, a.R, row);
+    if (r >= a.R) return;
+    int total, before;
+    tree_units<SLICE, COLS>(a, r, total, before);
+    const TreeRequest t = tree_request<SLICE, COLS>(a, r);
+    const int node = row - t.n0;
+    if (node < 0 || node >= t.nodes) return;
+    const int share = tree_share(total, a.blocks);
+    const float log2e = 1.4426950408889634f;
+    for (int head = wv; head < a.nq; head += 4) {
+        const int g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
+        const int u0 = before + group * t.slices, u1 = u0 + t.slices;
+        const int b0 = u0 / share, b1 = (u1 - 1) / share;
+        if (b0 == b1) continue;                  // (one block had all of it, and wrote the result)
+        float top = -INFINITY, sum = 0.f, acc[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = 0.f;
+        auto part_of = [&](int b) { return (((size_t)g * a.blocks + b) * 2 + (b == b0 && u0 != b * share ? 1 : 0)) * COLS + c; };
+        for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, a.part_ml[part_of(b) * 2]);
+        top = wave_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        for (int b = b0; b <= b1; ++b) {
+            const size_t p = part_of(b);
+            const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - ref);
+            sum += a.part_ml[p * 2 + 1] * f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] += a.part_o[p * D + i * 64 + lane] * f;
+        }
+        if (a.sinks) {
+            const float sink = a.sinks[head] * log2e;
+            if (top == -INFINITY) sum = 1.f;
+            else sum += __builtin_amdgcn_exp2f(sink - top);
+        }
+        const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
+        T* op = (T*)a.out + ((size_t)row * a.nq + head) * D;
+#pragma unroll
+        for (int i = 0; i < N; ++i) op[i * 64 + lane] = from_f32<T>(acc[i] * inv);
+    }
+}
+
+// The launch's shape: column tiles of a block and blocks a kv head; 0 tiles: the general kernel.
+struct TreePlan {
+    int tiles, blocks;
+};
+static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {
+    TreePlan p{0, 0};
+    if (!(d == 64 || d == 128 || d == 256) || page_size < 8 || (page_size & (page_size - 1)) || nkv <= 0 || nq % nkv || R <= 0 || rows <= 0) return p;
+    const int cols = (int)(((long long)rows * (nq / nkv) + R - 1) / R);      // a request's columns, on average
+    p.tiles = cols <= 16 ? 1 : cols <= 32 || d == 256 || dtype == TFF_F32 ? 2 : 4;
+    if (d == 256 && dtype == TFF_F32) p.tiles = 1;
+    const int slice = dtype == TFF_F32 ? 16 : 32;
+    const long long most = (long long)rows * (nq / nkv) / (16 * p.tiles) + R;     // groups of columns, at most
+    const long long units = most * (((long long)bt_stride * page_size + slice - 1) / slice);
+    if (units > 0x3fffffff) return TreePlan{0, 0};                                // (they are counted in 32 bits)
+    long long blocks = tff_device_cus() / nkv;
+    if (blocks < 1) blocks = 1;
+    p.blocks = (int)(blocks < (units + 7) / 8 ? blocks : (units + 7) / 8);
+    if (p.blocks < 1) p.blocks = 1;
+    return p;
+}
+TFF_API size_t tff_tree_attention_workspace_bytes(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {
+    const TreePlan p = tree_plan(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
+    return p.tiles ? (size_t)nkv * p.blocks * 2 * 16 * p.tiles * (d + 2) * 4 : 0;
+}
+
 TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const void* k_cache, const void* v_cache, const int32_t* block_tables,
                                int bt_stride, const int32_t* cu_nodes, const int32_t* start_pos, const int32_t* ancestors, int words, int R,
                                int rows, int nq, int nkv, int d, int page_size, int num_pages, int window, float scale, const float* sinks,
-                               float softcap, int dtype, tff_stream_t stream) {
+                               float softcap, void* workspace, size_t workspace_bytes, int dtype, tff_stream_t stream) {
     TFF_REQUIRE(rows >= 0 && R >= 0, "tree_attention: bad sizes rows=%d requests=%d", rows, R);
     TFF_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "tree_attention: %d query heads are not a multiple of %d key heads", nq, nkv);
     TFF_REQUIRE(nq <= 65535, "tree_attention: too many heads");
@@ -147,6 +712,45 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
     if (rows == 0 || R == 0) return 0;
     TFF_REQUIRE(q && out && k_cache && v_cache && block_tables && cu_nodes && start_pos && ancestors, "tree_attention: null pointer");
     hipStream_t s = (hipStream_t)stream;
+    const int esz = dtype == TFF_F32 ? 4 : 2;
+    const size_t need = tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
+    if (need > 0 && workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0 && ((uintptr_t)q & 15) == 0 &&
+        ((size_t)q_stride * esz) % 16 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0) {
+        const TreePlan p = tree_plan(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
+        int shift = 3;
+        for (int i = 3; i < 31; ++i)
+            if (page_size == 1 << i) shift = i;
+        float* part_o = (float*)workspace;
+        const TreeArgs a{q, k_cache, v_cache, out, block_tables, cu_nodes, start_pos, ancestors, sinks, part_o,
+                         part_o + (size_t)nkv * p.blocks * 2 * 16 * p.tiles * d, q_stride, bt_stride, words, R, rows, nq, nkv, page_size, shift,
+                         num_pages, window, p.blocks, scale, softcap};
+#define TFF_TREE_MM(TT, D, CT, OCC)                                                    \
+    do {                                                                               \
+        tree_attention_kernel<TT, D, CT, OCC><<<nkv * p.blocks, 256, 0, s>>>(a);       \
+        if (int rc = tff_check_launch("tree_attention")) return rc;                    \
+        tree_merge_kernel<TT, D, CT><<<rows, 256, 0, s>>>(a);                          \
+        return tff_check_launch("tree_merge");                                         \
+    } while (0)
+#define TFF_TREE_TILES(TT, D)                          \
+    do {                                               \
+        if (p.tiles == 1) TFF_TREE_MM(TT, D, 1, D == 256 ? 1 : 2);    \
+        if (p.tiles == 2) TFF_TREE_MM(TT, D, 2, D == 256 ? 1 : 2);    \
+    } while (0)
+        if (dtype == TFF_BF16) {
+            if (d == 64 && p.tiles == 4) TFF_TREE_MM(bf16_t, 64, 4, 1);
+            if (d == 128 && p.tiles == 4) TFF_TREE_MM(bf16_t, 128, 4, 1);
+            if (d == 64) TFF_TREE_TILES(bf16_t, 64);
+            if (d == 128) TFF_TREE_TILES(bf16_t, 128);
+            if (d == 256) TFF_TREE_TILES(bf16_t, 256);
+        } else {
+            if (d == 64) TFF_TREE_TILES(float, 64);
+            if (d == 128) TFF_TREE_TILES(float, 128);
+            if (d == 256) TFF_TREE_MM(float, 256, 1, 1);
+        }
+#undef TFF_TREE_TILES
+#undef TFF_TREE_MM
+        return tff_fail("tree_attention: no kernel for head size %d and %d column tiles", d, p.tiles);
+    }
     const dim3 grid(rows, nq);
 #define TFF_TREE(TT)                                                                                                                       \
     tree_attention_generic_kernel<TT><<<grid, 64, 0, s>>>((const TT*)q, q_stride, (TT*)out, (const TT*)k_cache, (const TT*)v_cache,       \

@@ -6,7 +6,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 
 from .build import ensure_built
 
-ABI_VERSION = 51
+ABI_VERSION = 52
 
 
 class KernelLibraryError(RuntimeError):
@@ -128,7 +128,8 @@ _SIGNATURES = {
     "tff_argmax": [_P, _P, _I, _I, _P, _P],
     "tff_repetition_penalty": [_P, _I, _I, _P, _P, _P, _P],
     "tff_adjust_logits": [_P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _P],
-    "tff_tree_attention": [_P, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _F, _I, _P],
+    "tff_tree_attention": [_P, _I, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _F, _P, _Z, _I, _P],
+    "tff_tree_attention_workspace_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
     "tff_tree_accept": [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P],
     "tff_cache_keep": [_P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "tff_sample": [_P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P],

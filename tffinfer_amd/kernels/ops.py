@@ -2734,10 +2734,14 @@ def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Te
     _one_device("tree_attention", q.device, k_cache, v_cache, block_tables, cu_nodes, start_pos, ancestors, sinks, out)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    _lib.check(_lib.load().tff_tree_attention(
+    L, code = _lib.load(), dtype_code(q.dtype)
+    room = L.tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, k_cache.shape[2], block_tables.stride(0), code)
+    ws = torch.empty(room // 4, dtype=torch.float32, device=q.device) if room else None
+    _lib.check(L.tff_tree_attention(
         q.data_ptr(), q.stride(0), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
         block_tables.stride(0), cu_nodes.data_ptr(), start_pos.data_ptr(), ancestors.data_ptr(), words, R, rows, nq, nkv, d,
-        k_cache.shape[2], k_cache.shape[0], int(window), float(scale), _ptr(sinks), float(softcap or 0.0), dtype_code(q.dtype), _stream()))
+        k_cache.shape[2], k_cache.shape[0], int(window), float(scale), _ptr(sinks), float(softcap or 0.0), _ptr(ws), room,
+        code, _stream()))
     return out
 
 
