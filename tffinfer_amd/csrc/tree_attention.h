@@ -1,0 +1,150 @@
+// What the kernels of drafted trees' attention share: what a node sees, and how blocks deal the work among themselves.
+#pragma once
+#include "common.h"
+
+#define TREE_WORDS 8                 // words of 32 bits a row of ancestors has at most: 256 nodes
+
+// The request that row t belongs to, the same in every lane: as many of cu[1 .. n] as are not behind t (n: to none).
+__device__ __forceinline__ int tree_row_request(const int32_t* __restrict__ cu, int n, int t) {
+    int upto = 0;
+    for (int r0 = 0; r0 < n; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        upto += __popcll(__ballot(r < n && cu[min(r, n - 1) + 1] <= t));
+    }
+    return upto;
+}
+
+// What a node sees of its tree (bits of nodes that the request has not are dropped, and under a window the first ones), and the first cached place.
+struct TreeRow {
+    uint32_t bits[TREE_WORDS];
+    int lo;
+};
+__device__ __forceinline__ TreeRow tree_row(const int32_t* __restrict__ row, int words, int nodes, int start, int window) {
+    TreeRow t;
+    int count = 0;
+#pragma unroll
+    for (int w = 0; w < TREE_WORDS; ++w) {
+        const int left = w < words ? nodes - 32 * w : 0;
+        t.bits[w] = (uint32_t)row[min(w, words - 1)] & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u);
+        count += __popc(t.bits[w]);
+    }
+    t.lo = 0;
+    if (window > 0) {
+        t.lo = max(0, min(start, start + count - window));
+        for (int drop = count - window; drop > 0; --drop) {      // (the window ends among the nodes)
+            bool done = false;
+#pragma unroll
+            for (int w = 0; w < TREE_WORDS; ++w) {
+                const uint32_t x = t.bits[w];
+                if (!done && x) {
+                    t.bits[w] = x & (x - 1);
+                    done = true;
+                }
+            }
+        }
+    }
+    return t;
+}
+
+struct TreeArgs {
+    const void *q, *k_cache, *v_cache;
+    void* out;
+    const int32_t *block_tables, *cu_nodes, *start_pos, *ancestors;
+    const float* sinks;
+    float *part_o, *part_ml;         // [kv head][block][2][columns][D], [..][columns][2]
+    int q_stride, bt_stride, words, R, rows, nq, nkv, page_size, page_shift, num_pages, window, blocks, least;
+    float scale, softcap;
+};
+
+// One request's share of the work.
+struct TreeRequest {
+    int n0, nodes, start, end, first;    // its first row, nodes, cached places, places, and the first place that a slice begins with
+    int slices, groups;
+};
+template <int SLICE, int COLS>
+__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
+    TreeRequest t;
+    t.n0 = max(a.cu_nodes[r], 0);
+    t.nodes = max(0, min(min(a.cu_nodes[r + 1], a.rows) - t.n0, 32 * a.words));
+    const long long room = (long long)a.bt_stride * a.page_size;
+    t.start = (int)min((long long)max(a.start_pos[r], 0), room);
+    t.end = (int)min((long long)t.start + t.nodes, room);
+    t.first = a.window > 0 ? max(0, t.start - a.window) / 32 * 32 : 0;
+    t.groups = (t.nodes * (a.nq / a.nkv) + COLS - 1) / COLS;
+    // (a request with nodes has a slice even where its table has no room for them: its rows are written)
+    t.slices = t.nodes > 0 ? max(1, (t.end - t.first + SLICE - 1) / SLICE) : 0;
+    return t;
+}
+__device__ __forceinline__ int tree_wave_scan(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v, o, 64);
+        if (lane >= o) v += up;
+    }
+    return v;
+}
+
+// Units of all requests, and of those before request `upto`; the same in every lane.
+template <int SLICE, int COLS>
+__device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& total, int& before) {
+    total = before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        const int r = r0 + (int)(threadIdx.x & 63);
+        int u = 0;
+        if (r < a.R) {
+            const TreeRequest t = tree_request<SLICE, COLS>(a, r);
+            u = t.slices * t.groups;
+        }
+        const int incl = tree_wave_scan(u);
+        if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
+}
+// How many units a block takes: an equal share, and no less than `least` (a block has its loads to wait for before the first).
+__device__ __forceinline__ int tree_share(int total, int blocks, int least) { return max((total + blocks - 1) / blocks, least); }
+
+// Block b's run of units u0 .. u1 - 1, the request that it begins in and the units before that request; the same in every lane.
+struct TreeRun {
+    int u0, u1, r, before;
+    TreeRequest t;
+};
+template <int SLICE, int COLS>
+__device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
+    const int lane = threadIdx.x & 63;
+    TreeRun run;
+    int total = 0, unused;
+    if (a.R > 64) tree_units<SLICE, COLS>(a, 0, total, unused);
+    run.r = run.before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
+        const int u = r0 + lane < a.R ? t.slices * t.groups : 0, incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
+        if (r0 == 0) {
+            if (a.R <= 64) total = all;
+            const int share = tree_share(total, a.blocks, a.least);
+            run.u0 = min(total, b * share);
+            run.u1 = min(total, run.u0 + share);
+        }
+        if (run.before + all <= run.u0) {
+            run.before += all;
+            continue;
+        }
+        const int at = __ffsll((long long)__ballot(run.before + incl > run.u0)) - 1;
+        run.r = r0 + at;
+        run.before += __builtin_amdgcn_readlane(incl - u, at);
+        run.t.n0 = __builtin_amdgcn_readlane(t.n0, at);
+        run.t.nodes = __builtin_amdgcn_readlane(t.nodes, at);
+        run.t.start = __builtin_amdgcn_readlane(t.start, at);
+        run.t.end = __builtin_amdgcn_readlane(t.end, at);
+        run.t.first = __builtin_amdgcn_readlane(t.first, at);
+        run.t.slices = __builtin_amdgcn_readlane(t.slices, at);
+        run.t.groups = __builtin_amdgcn_readlane(t.groups, at);
+        break;
+    }
+    return run;
+}
+
+// csrc/tree_attention_wide.hip: the plan's column tiles a wave (0: not its sizes), its launch
+int tree_wide_tiles(int columns, int d);
+int tree_wide_blocks_per_cu(int d, int tiles);
+int tree_wide_launch(const TreeArgs& a, int d, int tiles, hipStream_t stream);

@@ -7,51 +7,9 @@
 #include "common.h"
 #include "mfma_tiles.h"
 #include "tffinfer_kernels.h"
+#include "tree_attention.h"
 
-#define TREE_WORDS 8                 // words of 32 bits a row of ancestors has at most: 256 nodes
 #define TREE_MAX_D 512
-
-// The request that row t belongs to, the same in every lane: as many of cu[1 .. n] as are not behind t (n: to none).
-__device__ __forceinline__ int tree_row_request(const int32_t* __restrict__ cu, int n, int t) {
-    int upto = 0;
-    for (int r0 = 0; r0 < n; r0 += 64) {
-        const int r = r0 + (int)(threadIdx.x & 63);
-        upto += __popcll(__ballot(r < n && cu[min(r, n - 1) + 1] <= t));
-    }
-    return upto;
-}
-
-// What a node sees of its tree (bits of nodes that the request has not are dropped, and under a window the first ones), and the first cached place.
-struct TreeRow {
-    uint32_t bits[TREE_WORDS];
-    int lo;
-};
-__device__ __forceinline__ TreeRow tree_row(const int32_t* __restrict__ row, int words, int nodes, int start, int window) {
-    TreeRow t;
-    int count = 0;
-#pragma unroll
-    for (int w = 0; w < TREE_WORDS; ++w) {
-        const int left = w < words ? nodes - 32 * w : 0;
-        t.bits[w] = (uint32_t)row[min(w, words - 1)] & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u);
-        count += __popc(t.bits[w]);
-    }
-    t.lo = 0;
-    if (window > 0) {
-        t.lo = max(0, min(start, start + count - window));
-        for (int drop = count - window; drop > 0; --drop) {      // (the window ends among the nodes)
-            bool done = false;
-#pragma unroll
-            for (int w = 0; w < TREE_WORDS; ++w) {
-                const uint32_t x = t.bits[w];
-                if (!done && x) {
-                    t.bits[w] = x & (x - 1);
-                    done = true;
-                }
-            }
-        }
-    }
-    return t;
-}
 
 // ---- any head size, page size and type: a wave per (node, q head), keys 64 at a time, one a lane ----
 // The yardstick, and what sizes run on that the matrix cores' kernel does not take.
@@ -258,64 +216,6 @@ struct TreeMath<float, D> {
     }
 };
 
-struct TreeArgs {
-    const void *q, *k_cache, *v_cache;
-    void* out;
-    const int32_t *block_tables, *cu_nodes, *start_pos, *ancestors;
-    const float* sinks;
-    float *part_o, *part_ml;         // [kv head][block][2][columns][D], [..][columns][2]
-    int q_stride, bt_stride, words, R, rows, nq, nkv, page_size, page_shift, num_pages, window, blocks;
-    float scale, softcap;
-};
-
-// One request's share of the work.
-struct TreeRequest {
-    int n0, nodes, start, end, first;    // its first row, nodes, cached places, places, and the first place that a slice begins with
-    int slices, groups;
-};
-template <int SLICE, int COLS>
-__device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
-    TreeRequest t;
-    t.n0 = max(a.cu_nodes[r], 0);
-    t.nodes = max(0, min(min(a.cu_nodes[r + 1], a.rows) - t.n0, 32 * a.words));
-    const long long room = (long long)a.bt_stride * a.page_size;
-    t.start = (int)min((long long)max(a.start_pos[r], 0), room);
-    t.end = (int)min((long long)t.start + t.nodes, room);
-    t.first = a.window > 0 ? max(0, t.start - a.window) / 32 * 32 : 0;
-    t.groups = (t.nodes * (a.nq / a.nkv) + COLS - 1) / COLS;
-    // (a request with nodes has a slice even where its table has no room for them: its rows are written)
-    t.slices = t.nodes > 0 ? max(1, (t.end - t.first + SLICE - 1) / SLICE) : 0;
-    return t;
-}
-__device__ __forceinline__ int tree_wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(v, o, 64);
-        if (lane >= o) v += up;
-    }
-    return v;
-}
-// Units of all requests, and of those before request `upto`; the same in every lane.
-template <int SLICE, int COLS>
-__device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& total, int& before) {
-    total = before = 0;
-    for (int r0 = 0; r0 < a.R; r0 += 64) {
-        const int r = r0 + (int)(threadIdx.x & 63);
-        int u = 0;
-        if (r < a.R) {
-            const TreeRequest t = tree_request<SLICE, COLS>(a, r);
-            u = t.slices * t.groups;
-        }
-        const int incl = tree_wave_scan(u);
-        if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
-        total += __builtin_amdgcn_readlane(incl, 63);
-    }
-}
-// How many units a block takes: an equal share, and no less than two slices a wave (a wave that has one waits for memory once and then for
-// the other waves).
-__device__ __forceinline__ int tree_share(int total, int blocks) { return max((total + blocks - 1) / blocks, 8); }
-
 template <typename T, int D, int CT, int OCC>
 __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs a) {
     typedef TreeMath<T, D> M;
@@ -332,36 +232,16 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
     const float log2e = 1.4426950408889634f;
 
     // the block's run of units, and the request that it begins in
-    int total, before;
-    tree_units<SLICE, COLS>(a, 0, total, before);
-    const int share = tree_share(total, a.blocks), u0 = min(total, b * share), u1 = min(total, u0 + share);
+    const TreeRun run = tree_run<SLICE, COLS>(a, b);
+    const int u0 = run.u0, u1 = run.u1;
     if (u0 >= u1) return;
-    int r = 0;
-    before = 0;
-    for (int r0 = 0; r0 < a.R; r0 += 64) {
-        const int rr = r0 + lane;
-        int u = 0;
-        if (rr < a.R) {
-            const TreeRequest t = tree_request<SLICE, COLS>(a, rr);
-            u = t.slices * t.groups;
-        }
-        const int incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
-        if (before + all <= u0) {
-            before += all;
-            continue;
-        }
-        const int at = __ffsll((long long)__ballot(before + incl > u0)) - 1;
-        r = r0 + at;
-        before += at > 0 ? __builtin_amdgcn_readlane(incl, at - 1) : 0;
-        break;
-    }
+    int r = run.r, before = run.before;
+    TreeRequest t = run.t;
 
     for (int u = u0; u < u1;) {
-        const TreeRequest t = tree_request<SLICE, COLS>(a, r);
-        const int mine = t.slices * t.groups;
-        if (u >= before + mine) {
-            before += mine;
-            ++r;
+        if (u >= before + t.slices * t.groups) {
+            before += t.slices * t.groups;
+            t = tree_request<SLICE, COLS>(a, ++r);
             continue;
         }
         const int group = (u - before) / t.slices, s0 = u - before - group * t.slices;
@@ -626,74 +506,101 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
     }
 }
 
-// The partial results of a group of columns, in the order of the keys: a block a node, a wave a q head after the other.
-template <typename T, int D, int CT>
+// The partial results of a group of columns, in the order of the keys: a wave a (node, q head).
+template <typename T, int SLICE, int D, int COLS>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
-    constexpr int COLS = 16 * CT, SLICE = TreeMath<T, D>::SLICE, N = D / 64;
-    const int row = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6, G = a.nq / a.nkv;
-    const int r = tree_row_request(a.cu_nodes, a.R, row);
+    constexpr int N = D / 64;
+    const int row = blockIdx.x, lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6), G = a.nq / a.nkv;
+    if (head >= a.nq) return;
+    // the row's request, the units before it and all of them, in one pass over the tables
+    int r = 0, total = 0, before = 0;
+    for (int r0 = 0; r0 < a.R; r0 += 64) {
+        const TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
+        const bool in = r0 + lane < a.R;
+        const int u = in ? t.slices * t.groups : 0, incl = tree_wave_scan(u);
+        const int behind = __popcll(__ballot(in && a.cu_nodes[min(r0 + lane, a.R - 1) + 1] <= row));
+        if (r == r0) {
+            if (behind > 0) before += __builtin_amdgcn_readlane(incl, behind - 1);
+            r += behind;
+        }
+        total += __builtin_amdgcn_readlane(incl, 63);
+    }
     if (r >= a.R) return;
-    int total, before;
-    tree_units<SLICE, COLS>(a, r, total, before);
     const TreeRequest t = tree_request<SLICE, COLS>(a, r);
     const int node = row - t.n0;
     if (node < 0 || node >= t.nodes) return;
-    const int share = tree_share(total, a.blocks);
+    const int share = tree_share(total, a.blocks, a.least);
     const float log2e = 1.4426950408889634f;
-    for (int head = wv; head < a.nq; head += 4) {
-        const int g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
-        const int u0 = before + group * t.slices, u1 = u0 + t.slices;
-        const int b0 = u0 / share, b1 = (u1 - 1) / share;
-        if (b0 == b1) continue;                  // (one block had all of it, and wrote the result)
-        float top = -INFINITY, sum = 0.f, acc[N];
+    const int g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
+    const int u0 = before + group * t.slices, u1 = u0 + t.slices;
+    const int b0 = u0 / share, b1 = (u1 - 1) / share;
+    if (b0 == b1) return;                        // (one block had all of it, and wrote the result)
+    auto part_of = [&](int b) { return (((size_t)g * a.blocks + b) * 2 + (b == b0 && u0 != b * share ? 1 : 0)) * COLS + c; };
+    float top = -INFINITY, sum = 0.f, acc[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] = 0.f;
-        auto part_of = [&](int b) { return (((size_t)g * a.blocks + b) * 2 + (b == b0 && u0 != b * share ? 1 : 0)) * COLS + c; };
-        for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, a.part_ml[part_of(b) * 2]);
-        top = wave_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        for (int b = b0; b <= b1; ++b) {
-            const size_t p = part_of(b);
-            const float f = __builtin_amdgcn_exp2f(a.part_ml[p * 2] - ref);
-            sum += a.part_ml[p * 2 + 1] * f;
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, a.part_ml[part_of(b) * 2]);
+    top = wave_max(top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    for (int c0 = b0; c0 <= b1; c0 += 64) {
+        const int n = min(64, b1 - c0 + 1);
+        const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[part_of(c0 + min(lane, n - 1))];
+        const float f = lane < n ? __builtin_amdgcn_exp2f(ml.x - ref) : 0.f;
+        sum += wave_sum(lane < n ? ml.y * f : 0.f);
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const float w = __shfl(f, i, 64);
+            const float* o = a.part_o + part_of(c0 + i) * D + lane;
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] += a.part_o[p * D + i * 64 + lane] * f;
+            for (int k = 0; k < N; ++k) acc[k] += o[k * 64] * w;
         }
-        if (a.sinks) {
-            const float sink = a.sinks[head] * log2e;
-            if (top == -INFINITY) sum = 1.f;
-            else sum += __builtin_amdgcn_exp2f(sink - top);
-        }
-        const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
-        T* op = (T*)a.out + ((size_t)row * a.nq + head) * D;
-#pragma unroll
-        for (int i = 0; i < N; ++i) op[i * 64 + lane] = from_f32<T>(acc[i] * inv);
     }
+    if (a.sinks) {
+        const float sink = a.sinks[head] * log2e;
+        if (top == -INFINITY) sum = 1.f;
+        else sum += __builtin_amdgcn_exp2f(sink - top);
+    }
+    const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
+    T* op = (T*)a.out + ((size_t)row * a.nq + head) * D;
+#pragma unroll
+    for (int i = 0; i < N; ++i) op[i * 64 + lane] = from_f32<T>(acc[i] * inv);
 }
 
-// The launch's shape: column tiles of a block and blocks a kv head; 0 tiles: the general kernel.
+// The launch's shape: column tiles of a block (narrow: all of them in every wave; wide: of each wave), blocks a kv head, units a block
+// takes at least; 0 tiles: the general kernel.
 struct TreePlan {
-    int tiles, blocks;
+    int wide, tiles, blocks, least, columns;
 };
 static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {
-    TreePlan p{0, 0};
-    if (!(d == 64 || d == 128 || d == 256) || page_size < 8 || (page_size & (page_size - 1)) || nkv <= 0 || nq % nkv || R <= 0 || rows <= 0) return p;
+    TreePlan p{0, 0, 0, 0, 0};
+    if (!(d == 64 || d == 128 || d == 256) || page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || nkv <= 0 || nq % nkv || R <= 0 || rows <= 0) return p;
     const int cols = (int)(((long long)rows * (nq / nkv) + R - 1) / R);      // a request's columns, on average
-    p.tiles = cols <= 16 ? 1 : cols <= 32 || d == 256 || dtype == TFF_F32 ? 2 : 4;
-    if (d == 256 && dtype == TFF_F32) p.tiles = 1;
+    int per_cu = 1;
+    if (dtype == TFF_BF16 && tree_wide_tiles(cols, d) > 0) {
+        p.wide = 1;
+        p.tiles = tree_wide_tiles(cols, d);
+        p.columns = 64 * p.tiles;
+        per_cu = tree_wide_blocks_per_cu(d, p.tiles);
+        p.least = 4;
+    } else {
+        p.tiles = cols <= 16 || (d == 256 && dtype == TFF_F32) ? 1 : 2;
+        p.columns = 16 * p.tiles;
+        if (d < 256) per_cu = 2;
+        p.least = 8;
+    }
     const int slice = dtype == TFF_F32 ? 16 : 32;
-    const long long most = (long long)rows * (nq / nkv) / (16 * p.tiles) + R;     // groups of columns, at most
+    const long long most = (long long)rows * (nq / nkv) / p.columns + R;     // groups of columns, at most
     const long long units = most * (((long long)bt_stride * page_size + slice - 1) / slice);
-    if (units > 0x3fffffff) return TreePlan{0, 0};                                // (they are counted in 32 bits)
-    long long blocks = tff_device_cus() / nkv;
+    if (units > 0x3fffffff) return TreePlan{0, 0, 0, 0, 0};                  // (they are counted in 32 bits)
+    long long blocks = (long long)tff_device_cus() * per_cu / nkv;
     if (blocks < 1) blocks = 1;
-    p.blocks = (int)(blocks < (units + 7) / 8 ? blocks : (units + 7) / 8);
+    p.blocks = (int)(blocks < (units + p.least - 1) / p.least ? blocks : (units + p.least - 1) / p.least);
     if (p.blocks < 1) p.blocks = 1;
     return p;
 }
 TFF_API size_t tff_tree_attention_workspace_bytes(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {
     const TreePlan p = tree_plan(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
-    return p.tiles ? (size_t)nkv * p.blocks * 2 * 16 * p.tiles * (d + 2) * 4 : 0;
+    return p.tiles ? (size_t)nkv * p.blocks * 2 * p.columns * (d + 2) * 4 : 0;
 }
 
 TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const void* k_cache, const void* v_cache, const int32_t* block_tables,
@@ -722,34 +629,50 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
             if (page_size == 1 << i) shift = i;
         float* part_o = (float*)workspace;
         const TreeArgs a{q, k_cache, v_cache, out, block_tables, cu_nodes, start_pos, ancestors, sinks, part_o,
-                         part_o + (size_t)nkv * p.blocks * 2 * 16 * p.tiles * d, q_stride, bt_stride, words, R, rows, nq, nkv, page_size, shift,
-                         num_pages, window, p.blocks, scale, softcap};
-#define TFF_TREE_MM(TT, D, CT, OCC)                                                    \
-    do {                                                                               \
-        tree_attention_kernel<TT, D, CT, OCC><<<nkv * p.blocks, 256, 0, s>>>(a);       \
-        if (int rc = tff_check_launch("tree_attention")) return rc;                    \
-        tree_merge_kernel<TT, D, CT><<<rows, 256, 0, s>>>(a);                          \
-        return tff_check_launch("tree_merge");                                         \
+                         part_o + (size_t)nkv * p.blocks * 2 * p.columns * d, q_stride, bt_stride, words, R, rows, nq, nkv, page_size, shift,
+                         num_pages, window, p.blocks, p.least, scale, softcap};
+        const dim3 merge(rows, (nq + 3) / 4);
+#define TFF_TREE_MERGE(TT, SL, D, COLS)                                       \
+    do {                                                                      \
+        tree_merge_kernel<TT, SL, D, COLS><<<merge, 256, 0, s>>>(a);          \
+        return tff_check_launch("tree_merge");                                \
     } while (0)
-#define TFF_TREE_TILES(TT, D)                          \
-    do {                                               \
-        if (p.tiles == 1) TFF_TREE_MM(TT, D, 1, D == 256 ? 1 : 2);    \
-        if (p.tiles == 2) TFF_TREE_MM(TT, D, 2, D == 256 ? 1 : 2);    \
+#define TFF_TREE_MM(TT, SL, D, CT, OCC)                                              \
+    do {                                                                             \
+        tree_attention_kernel<TT, D, CT, OCC><<<nkv * p.blocks, 256, 0, s>>>(a);     \
+        if (int rc = tff_check_launch("tree_attention")) return rc;                  \
+        TFF_TREE_MERGE(TT, SL, D, 16 * CT);                                          \
+    } while (0)
+        if (p.wide) {
+            if (int rc = tree_wide_launch(a, d, p.tiles, s)) return rc;
+#define TFF_TREE_WIDE(D)                                                      \
+    do {                                                                      \
+        if (p.tiles == 1) TFF_TREE_MERGE(bf16_t, 32, D, 64);                  \
+        if (p.tiles == 2) TFF_TREE_MERGE(bf16_t, 32, D, 128);                 \
+        TFF_TREE_MERGE(bf16_t, 32, D, 256);                                   \
+    } while (0)
+            if (d == 64) TFF_TREE_WIDE(64);
+            if (d == 128) TFF_TREE_WIDE(128);
+            TFF_TREE_WIDE(256);
+#undef TFF_TREE_WIDE
+        }
+#define TFF_TREE_TILES(TT, SL)                                   \
+    do {                                                         \
+        if (d == 64 && p.tiles == 1) TFF_TREE_MM(TT, SL, 64, 1, 2);   \
+        if (d == 64) TFF_TREE_MM(TT, SL, 64, 2, 2);              \
+        if (d == 128 && p.tiles == 1) TFF_TREE_MM(TT, SL, 128, 1, 2); \
+        if (d == 128) TFF_TREE_MM(TT, SL, 128, 2, 2);            \
+        if (p.tiles == 1) TFF_TREE_MM(TT, SL, 256, 1, 1);        \
     } while (0)
         if (dtype == TFF_BF16) {
-            if (d == 64 && p.tiles == 4) TFF_TREE_MM(bf16_t, 64, 4, 1);
-            if (d == 128 && p.tiles == 4) TFF_TREE_MM(bf16_t, 128, 4, 1);
-            if (d == 64) TFF_TREE_TILES(bf16_t, 64);
-            if (d == 128) TFF_TREE_TILES(bf16_t, 128);
-            if (d == 256) TFF_TREE_TILES(bf16_t, 256);
-        } else {
-            if (d == 64) TFF_TREE_TILES(float, 64);
-            if (d == 128) TFF_TREE_TILES(float, 128);
-            if (d == 256) TFF_TREE_MM(float, 256, 1, 1);
+            TFF_TREE_TILES(bf16_t, 32);
+            TFF_TREE_MM(bf16_t, 32, 256, 2, 1);
         }
+        TFF_TREE_TILES(float, 16);
+        return tff_fail("tree_attention: no kernel for head size %d and %d column tiles", d, p.tiles);
 #undef TFF_TREE_TILES
 #undef TFF_TREE_MM
-        return tff_fail("tree_attention: no kernel for head size %d and %d column tiles", d, p.tiles);
+#undef TFF_TREE_MERGE
     }
     const dim3 grid(rows, nq);
 #define TFF_TREE(TT)                                                                                                                       \
