@@ -44,18 +44,29 @@ __device__ __forceinline__ int row_request(const int32_t* __restrict__ cu, int n
     return upto;
 }
 
+// Four bits of a mask from token v on (the words behind the last are not read).
+__device__ __forceinline__ uint32_t mask_bits4(const int32_t* __restrict__ mask, int words, int v) {
+    const int w = v >> 5;
+    return __funnelshift_r((uint32_t)mask[w], (uint32_t)mask[min(w + 1, words - 1)], v & 31);
+}
+
+// RUN tokens of one row for a block of 256 threads, RUN / 1024 groups of four a thread.  A row need not begin at a multiple of 16 bytes: the groups
+// do, and up to three tokens before the first and behind the last are the first threads' besides.
 template <int RUN>
-__global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) {
-    __shared__ uint32_t cnt[RUN];
+__global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, const int vec) {
+    constexpr int PER = RUN / 1024;
+    __shared__ __attribute__((aligned(16))) uint32_t cnt[RUN];
+    __shared__ uint32_t touched[RUN / 32];       // which tokens have a count
     const int t = blockIdx.x / a.runs, v0 = (blockIdx.x - t * a.runs) * RUN, n = min(RUN, a.V - v0), tid = threadIdx.x;
     const size_t base = (size_t)t * a.V + v0;
-    const float* __restrict__ x = a.logits + base;
-    float* __restrict__ y = a.out + base;
+    const float* x = a.logits + base;
+    float* y = a.out + base;                     // (may be x)
     const bool in_place = a.logits == a.out;
+    const int mask_row = a.mask_rows ? a.mask_rows[t] : -1;
     int r = t;
     if (a.cu_nodes) r = row_request(a.cu_nodes, a.requests, t);
+    r = __builtin_amdgcn_readfirstlane(r);
     const bool has_request = r < a.requests;      // (a row behind the last node is left as it is)
-    const int mask_row = a.mask_rows ? a.mask_rows[t] : -1;
     const int32_t* __restrict__ mask = has_request && mask_row >= 0 && mask_row < a.num_masks ? a.masks + (size_t)mask_row * a.mask_words : nullptr;
     float rep = 1.f, pres = 0.f, freq = 0.f;
     if (has_request) {
@@ -64,43 +75,102 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) 
         freq = a.frequency[r];
     }
     const bool counts = rep != 1.f || pres != 0.f || freq != 0.f;
+    const int head = vec ? min(n, (int)(-base & 3)) : n, groups = (n - head) / 4;      // (without `vec` all are the first threads' besides)
+
+    // the logits and their bits are on their way while the history is counted
+    float4 v[PER];
+    uint32_t allowed[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int j = tid + 256 * k;
+        allowed[k] = 15u;
+        if (mask && j < groups) allowed[k] = mask_bits4(mask, a.mask_words, v0 + head + 4 * j) & 15u;
+    }
+    if (!in_place) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int j = tid + 256 * k;
+            if (j < groups && allowed[k]) v[k] = *reinterpret_cast<const float4*>(x + head + 4 * j);
+        }
+    }
     if (counts) {
-        for (int i = tid; i < n; i += 256) cnt[i] = 0;
+        for (int i = tid; i < RUN / 4; i += 256) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < RUN / 32; i += 256) touched[i] = 0;
         __syncthreads();
+        auto count = [&](int token, bool output) {
+            const int at = token - v0;
+            if (at >= 0 && at < n) {
+                if (output) atomicAdd(&cnt[at], 1u);
+                else atomicOr(&cnt[at], ADJUST_SEEN);
+                atomicOr(&touched[at >> 5], 1u << (at & 31));
+            }
+        };
         const int h0 = min(max(a.cu_history[r], 0), a.history_len), h1 = min(max(a.cu_history[r + 1], h0), a.history_len);
         const int out0 = h0 + min(max(a.prompt_lens[r], 0), h1 - h0);
-        for (int i = h0 + tid; i < h1; i += 256) {
-            const int at = a.history[i] - v0;
-            if (at >= 0 && at < n) {
-                if (i < out0) atomicOr(&cnt[at], ADJUST_SEEN);
-                else atomicAdd(&cnt[at], 1u);
+        const int q0 = min(h1, (h0 + 3) & ~3), q1 = max(q0, h1 & ~3);      // (the part that int4 loads can take)
+        const bool hvec = ((uintptr_t)a.history & 15) == 0;
+        if (hvec) {
+            for (int i = q0 / 4 + tid; i < q1 / 4; i += 256) {
+                const int4 h = reinterpret_cast<const int4*>(a.history)[i];
+                count(h.x, 4 * i >= out0);
+                count(h.y, 4 * i + 1 >= out0);
+                count(h.z, 4 * i + 2 >= out0);
+                count(h.w, 4 * i + 3 >= out0);
             }
+            if (tid < 8) {
+                const int i = tid < 4 ? h0 + tid : q1 + tid - 4;
+                if (tid < 4 ? i < q0 : i < h1) count(a.history[i], i >= out0);
+            }
+        } else {
+            for (int i = h0 + tid; i < h1; i += 256) count(a.history[i], i >= out0);
         }
         if (a.cu_nodes) {
             const int n0 = max(a.cu_nodes[r], 0), nodes = min(min(a.cu_nodes[r + 1], a.rows) - n0, 32 * a.words);
             for (int j = tid; j < nodes; j += 256)
-                if ((a.ancestors[(size_t)t * a.words + (j >> 5)] >> (j & 31)) & 1) {
-                    const int at = a.draft_tokens[n0 + j] - v0;
-                    if (at >= 0 && at < n) atomicAdd(&cnt[at], 1u);
-                }
+                if ((a.ancestors[(size_t)t * a.words + (j >> 5)] >> (j & 31)) & 1) count(a.draft_tokens[n0 + j], true);
         }
         __syncthreads();
     }
-    for (int i = tid; i < n; i += 256) {
-        const bool allowed = !mask || ((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1);
-        const uint32_t c = counts ? cnt[i] : 0u;
-        if (!allowed) {
-            y[i] = -INFINITY;
-        } else if (c || !in_place) {
-            float v = x[i];
-            if (c) {
-                v = v > 0.f ? v / rep : v * rep;
-                const uint32_t k = c & ~ADJUST_SEEN;
-                if (k) v = v - freq * (float)k - pres;
-            }
-            y[i] = v;
+    auto adjusted = [&](float z, uint32_t c) {
+        if (c) {
+            z = z > 0.f ? z / rep : z * rep;
+            const uint32_t k = c & ~ADJUST_SEEN;
+            if (k) z = z - freq * (float)k - pres;
         }
+        return z;
+    };
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int j = tid + 256 * k, i = head + 4 * j;
+        if (j >= groups) continue;
+        uint32_t some = 0;
+        if (counts) some = __funnelshift_r(touched[i >> 5], touched[min((i >> 5) + 1, RUN / 32 - 1)], i & 31) & 15u;
+        if (in_place && allowed[k] == 15u && !some) continue;
+        float4 z = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (allowed[k]) {
+            z = v[k];
+            if (in_place) z = *reinterpret_cast<const float4*>(x + i);
+            if (some) {
+                z.x = adjusted(z.x, cnt[i]);
+                z.y = adjusted(z.y, cnt[i + 1]);
+                z.z = adjusted(z.z, cnt[i + 2]);
+                z.w = adjusted(z.w, cnt[i + 3]);
+            }
+            if (!(allowed[k] & 1)) z.x = -INFINITY;
+            if (!(allowed[k] & 2)) z.y = -INFINITY;
+            if (!(allowed[k] & 4)) z.z = -INFINITY;
+            if (!(allowed[k] & 8)) z.w = -INFINITY;
+        }
+        *reinterpret_cast<float4*>(y + i) = z;
     }
+    auto one = [&](int i) {
+        const bool may = !mask || ((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1);
+        const uint32_t c = counts ? cnt[i] : 0u;
+        if (!may) y[i] = -INFINITY;
+        else if (c || !in_place) y[i] = adjusted(x[i], c);
+    };
+    for (int i = tid; i < head; i += 256) one(i);
+    for (int i = head + 4 * groups + tid; i < n; i += 256) one(i);
     if (a.cu_bias && has_request) {
         // of equal tokens the last one listed counts: the largest place among them wins, by an integer maximum
         const int b0 = min(max(a.cu_bias[r], 0), a.bias_len), b1 = min(max(a.cu_bias[r + 1], b0), a.bias_len);
@@ -117,8 +187,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a) 
             }
             __syncthreads();
             for (int i = b0 + tid; i < b1; i += 256) {
-                const int v = a.bias_ids[i], at = v - v0;
-                if (at >= 0 && at < n && cnt[at] == (uint32_t)(i - b0 + 1) && (!mask || ((mask[v >> 5] >> (v & 31)) & 1))) y[at] += a.bias_values[i];
+                const int z = a.bias_ids[i], at = z - v0;
+                if (at >= 0 && at < n && cnt[at] == (uint32_t)(i - b0 + 1) && (!mask || ((mask[z >> 5] >> (z & 31)) & 1))) y[at] += a.bias_values[i];
             }
         }
     }
@@ -138,10 +208,14 @@ TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, 
     TFF_REQUIRE(!mask_rows || num_masks == 0 || masks, "adjust_logits: rows with masks, and no masks");
     TFF_REQUIRE(!cu_nodes || (draft_tokens && ancestors && words > 0), "adjust_logits: nodes without their tokens and ancestors");
     TFF_REQUIRE(cu_nodes || rows == requests, "adjust_logits: %d rows of %d requests", rows, requests);
-    const int run = 8192, runs = (V + run - 1) / run;
+    // Runs of 8,192 tokens, or of 2,048 where those would leave CUs without a block: every run goes through the request's whole history, so few and
+    // long ones are better as soon as they fill the chip.
+    const int run = (int64_t)rows * ((V + 8191) / 8192) >= tff_device_cus() ? 8192 : 2048, runs = (V + run - 1) / run;
     TFF_REQUIRE((int64_t)rows * runs <= 0x7fffffff, "adjust_logits: %d rows of %d logits are more than a launch takes", rows, V);
     const AdjustArgs a{logits, out, rows, V, runs, history, cu_history, prompt_lens, history_len, requests, repetition, presence, frequency,
                        bias_ids, bias_values, cu_bias, bias_len, masks, masks ? num_masks : 0, (V + 31) / 32, mask_rows, draft_tokens, cu_nodes, ancestors, words};
-    adjust_logits_kernel<8192><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a);
+    const int vec = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0;      // (rows of both then begin alike)
+    if (run == 8192) adjust_logits_kernel<8192><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a, vec);
+    else adjust_logits_kernel<2048><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a, vec);
     return tff_check_launch("adjust_logits");
 }
