@@ -104,6 +104,15 @@ __device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& tot
 // How many units a block takes: an equal share, and no less than `least` (a block has its loads to wait for before the first).
 __device__ __forceinline__ int tree_share(int total, int blocks, int least) { return max((total + blocks - 1) / blocks, least); }
 
+// Which run and kv head a block of the launch has: eight runs by eight, within them the kv heads, within a kv head the eight runs.  Blocks go
+// to the XCDs in turn, so a run's kv heads are on one XCD and a page of keys is read through one L2 and one address translation.
+__device__ __forceinline__ void tree_place(int nkv, int& b, int& g) {
+    const int eight = blockIdx.x / (8 * nkv), within = blockIdx.x - eight * (8 * nkv);
+    b = eight * 8 + (within & 7);
+    g = within >> 3;
+}
+static inline int tree_grid(int nkv, int blocks) { return nkv * ((blocks + 7) / 8 * 8); }
+
 // Block b's run of units u0 .. u1 - 1, the request that it begins in and the units before that request; the same in every lane.
 struct TreeRun {
     int u0, u1, r, before;

@@ -225,7 +225,10 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
     __shared__ float merge_m[4 * COLS], merge_l[4 * COLS];
     __shared__ uint32_t see[COLS * (TREE_WORDS + 1)];                        // the columns' bits, and a word of zeros
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), qc = lane & 15, kg = lane >> 4;
-    const int g = blockIdx.x % a.nkv, b = blockIdx.x / a.nkv, G = a.nq / a.nkv;
+    const int G = a.nq / a.nkv;
+    int b, g;
+    tree_place(a.nkv, b, g);
+    if (b >= a.blocks) return;
     const size_t page_stride = (size_t)a.nkv * a.page_size * D;
     const T* __restrict__ kc = (const T*)a.k_cache + (size_t)g * a.page_size * D;
     const T* __restrict__ vc = (const T*)a.v_cache + (size_t)g * a.page_size * D;
@@ -248,56 +251,6 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
         const int s1 = min(t.slices, s0 + (u1 - u));
         const int ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
-
-        // the columns: queries, bits, the first cached place of each
-        frag q[CT][M::QF];
-        int lo[CT], lo_least = t.end, lo_most = 0;
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            const int c = min(ct * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
-            const T* qp = (const T*)a.q + (size_t)(t.n0 + node) * a.q_stride + (size_t)head * D;
-#pragma unroll
-            for (int f = 0; f < M::QF; ++f) q[ct][f] = *reinterpret_cast<const frag*>(qp + M::key_elem(f, kg));
-            lo[ct] = 0;
-        }
-        __syncthreads();                 // (the run before is merged)
-        for (int c = tid; c < COLS; c += 256) {
-            const int node = (min(c, ncols - 1) + group * COLS) / G;
-            const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + node) * a.words, a.words, t.end - t.start, t.start, a.window);
-#pragma unroll
-            for (int w = 0; w < TREE_WORDS; ++w) see[c * (TREE_WORDS + 1) + w] = row.bits[w];
-            see[c * (TREE_WORDS + 1) + TREE_WORDS] = 0;
-            merge_m[c] = __int_as_float(row.lo);
-        }
-        __syncthreads();
-        if (a.window > 0) {
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                lo[ct] = __float_as_int(merge_m[ct * 16 + qc]);
-                lo_least = min(lo_least, lo[ct]);
-                lo_most = max(lo_most, lo[ct]);
-            }
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) {
-                lo_least = min(lo_least, __shfl_xor(lo_least, o, 64));
-                lo_most = max(lo_most, __shfl_xor(lo_most, o, 64));
-            }
-            lo_least = __builtin_amdgcn_readfirstlane(lo_least);
-            lo_most = __builtin_amdgcn_readfirstlane(lo_most);
-            __syncthreads();             // (merge_m is written at the run's end)
-        } else {
-            lo_least = 0;
-        }
-
-        tree_f32x4 o[CT][D / 16];
-        float m[CT], l[CT];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            m[ct] = -INFINITY;
-            l[ct] = 0.f;
-#pragma unroll
-            for (int dt = 0; dt < D / 16; ++dt) o[ct][dt] = tree_f32x4{0.f, 0.f, 0.f, 0.f};
-        }
 
         // places of slice s that a lane loads from: pages two slices ahead, so that no load of a page number waits behind keys and values
         const int last_block = (max(t.end, 1) - 1) >> 3;         // blocks of eight places lie in one page
@@ -325,6 +278,63 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
             }
         };
 
+        // The first slice's page numbers, the queries and the columns' bits are asked for together, then the keys and values; the rest of what a run
+        // begins with is done while they travel.
+        int s = s0 + wv;
+        const int pk0 = page_of(place(s, kb)), pv0 = page_of(place(s, vb));
+        int pk = page_of(place(s + 4, kb)), pv = page_of(place(s + 4, vb));
+        frag q[CT][M::QF];
+        int lo[CT], lo_least = t.end, lo_most = 0;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            const int c = min(ct * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
+            const T* qp = (const T*)a.q + (size_t)(t.n0 + node) * a.q_stride + (size_t)head * D;
+#pragma unroll
+            for (int f = 0; f < M::QF; ++f) q[ct][f] = *reinterpret_cast<const frag*>(qp + M::key_elem(f, kg));
+            lo[ct] = 0;
+        }
+        static_assert(COLS <= 64, "a lane a column");
+        const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + (min(lane, ncols - 1) + group * COLS) / G) * a.words, a.words, t.end - t.start,
+                                     t.start, a.window);
+        if (s < s1) {
+            load_k(s, pk0);
+            load_v(s, pv0);
+        }
+        __syncthreads();                 // (the run before is merged)
+        if (tid < COLS) {
+#pragma unroll
+            for (int w = 0; w < TREE_WORDS; ++w) see[tid * (TREE_WORDS + 1) + w] = row.bits[w];
+            see[tid * (TREE_WORDS + 1) + TREE_WORDS] = 0;
+        }
+        __syncthreads();
+        if (a.window > 0) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                lo[ct] = __shfl(row.lo, ct * 16 + qc, 64);
+                lo_least = min(lo_least, lo[ct]);
+                lo_most = max(lo_most, lo[ct]);
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                lo_least = min(lo_least, __shfl_xor(lo_least, o, 64));
+                lo_most = max(lo_most, __shfl_xor(lo_most, o, 64));
+            }
+            lo_least = __builtin_amdgcn_readfirstlane(lo_least);
+            lo_most = __builtin_amdgcn_readfirstlane(lo_most);
+        } else {
+            lo_least = 0;
+        }
+
+        tree_f32x4 o[CT][D / 16];
+        float m[CT], l[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            m[ct] = -INFINITY;
+            l[ct] = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < D / 16; ++dt) o[ct][dt] = tree_f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
         // which of the places key, key + 1, ... column ct * 16 + qc sees: a bit each (the next 8 of them hold)
         auto visible = [&](int ct, int key) {
             const int j = key - t.start;
@@ -339,13 +349,6 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
 
         // A slice's keys are asked for as soon as the slice before is multiplied, its values as soon as that one's are: either is on its way while
         // the wave works on the other, in one set of registers.
-        int s = s0 + wv, pk = 0, pv = 0;
-        if (s < s1) {
-            load_k(s, page_of(place(s, kb)));
-            load_v(s, page_of(place(s, vb)));
-            pk = page_of(place(s + 4, kb));
-            pv = page_of(place(s + 4, vb));
-        }
         for (; s < s1; s += 4) {
             const int k0 = t.first + s * SLICE;
             const bool masked = k0 + SLICE > t.start || k0 < lo_most;
@@ -547,12 +550,19 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
         const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[part_of(c0 + min(lane, n - 1))];
         const float f = lane < n ? __builtin_amdgcn_exp2f(ml.x - ref) : 0.f;
         sum += wave_sum(lane < n ? ml.y * f : 0.f);
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const float w = __shfl(f, i, 64);
-            const float* o = a.part_o + part_of(c0 + i) * D + lane;
+        for (int i0 = 0; i0 < n; i0 += 4) {      // (four at a time: their loads together)
+            float o[4][N], w[4];
 #pragma unroll
-            for (int k = 0; k < N; ++k) acc[k] += o[k * 64] * w;
+            for (int i = 0; i < 4; ++i) {
+                const float* p = a.part_o + part_of(c0 + min(i0 + i, n - 1)) * D + lane;
+#pragma unroll
+                for (int k = 0; k < N; ++k) o[i][k] = p[k * 64];
+                w[i] = i0 + i < n ? __shfl(f, min(i0 + i, 63), 64) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[k] += i0 + i < n ? o[i][k] * w[i] : 0.f;
         }
     }
     if (a.sinks) {
@@ -583,13 +593,14 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
         per_cu = tree_wide_blocks_per_cu(d, p.tiles);
         p.least = 4;
     } else {
-        p.tiles = cols <= 16 || (d == 256 && dtype == TFF_F32) ? 1 : 2;
+        p.tiles = cols <= 16 || d == 256 ? 1 : 2;      // (two tiles of a head of 256 are more than the registers hold)
         p.columns = 16 * p.tiles;
         if (d < 256) per_cu = 2;
-        p.least = 8;
+        // slices a wave: four where they are quick (a run that one block has whole needs no merge), one where float32's are not (2 us each)
+        p.least = dtype == TFF_F32 ? 4 : 16;
     }
     const int slice = dtype == TFF_F32 ? 16 : 32;
-    const long long most = (long long)rows * (nq / nkv) / p.columns + R;     // groups of columns, at most
+    const long long all = (long long)rows * (nq / nkv), most = (all > R ? all - R : 0) / p.columns + R;      // groups of columns, at most
     const long long units = most * (((long long)bt_stride * page_size + slice - 1) / slice);
     if (units > 0x3fffffff) return TreePlan{0, 0, 0, 0, 0};                  // (they are counted in 32 bits)
     long long blocks = (long long)tff_device_cus() * per_cu / nkv;
@@ -632,14 +643,16 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
                          part_o + (size_t)nkv * p.blocks * 2 * p.columns * d, q_stride, bt_stride, words, R, rows, nq, nkv, page_size, shift,
                          num_pages, window, p.blocks, p.least, scale, softcap};
         const dim3 merge(rows, (nq + 3) / 4);
+        // (a block a kv head has every run whole)
 #define TFF_TREE_MERGE(TT, SL, D, COLS)                                       \
     do {                                                                      \
+        if (p.blocks == 1) return 0;                                          \
         tree_merge_kernel<TT, SL, D, COLS><<<merge, 256, 0, s>>>(a);          \
         return tff_check_launch("tree_merge");                                \
     } while (0)
 #define TFF_TREE_MM(TT, SL, D, CT, OCC)                                              \
     do {                                                                             \
-        tree_attention_kernel<TT, D, CT, OCC><<<nkv * p.blocks, 256, 0, s>>>(a);     \
+        tree_attention_kernel<TT, D, CT, OCC><<<tree_grid(nkv, p.blocks), 256, 0, s>>>(a); \
         if (int rc = tff_check_launch("tree_attention")) return rc;                  \
         TFF_TREE_MERGE(TT, SL, D, 16 * CT);                                          \
     } while (0)
@@ -662,14 +675,10 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
         if (d == 64) TFF_TREE_MM(TT, SL, 64, 2, 2);              \
         if (d == 128 && p.tiles == 1) TFF_TREE_MM(TT, SL, 128, 1, 2); \
         if (d == 128) TFF_TREE_MM(TT, SL, 128, 2, 2);            \
-        if (p.tiles == 1) TFF_TREE_MM(TT, SL, 256, 1, 1);        \
+        TFF_TREE_MM(TT, SL, 256, 1, 1);                          \
     } while (0)
-        if (dtype == TFF_BF16) {
-            TFF_TREE_TILES(bf16_t, 32);
-            TFF_TREE_MM(bf16_t, 32, 256, 2, 1);
-        }
+        if (dtype == TFF_BF16) TFF_TREE_TILES(bf16_t, 32);
         TFF_TREE_TILES(float, 16);
-        return tff_fail("tree_attention: no kernel for head size %d and %d column tiles", d, p.tiles);
 #undef TFF_TREE_TILES
 #undef TFF_TREE_MM
 #undef TFF_TREE_MERGE

@@ -37,6 +37,13 @@ __device__ __forceinline__ void copy16_off(unsigned long long g, unsigned lds) {
 }
 // an accumulator stays in its register class, and what follows reads it here
 __device__ __forceinline__ void pin(floatx4& x) { asm volatile("" : "+a"(x)); }
+// (as an instruction: the compiler would quiet every operand first)
+__device__ __forceinline__ float largest3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ void to_acc(bf16x8& x) { asm volatile("" : "+a"(x)); }
 __device__ __forceinline__ void hold(bf16x8& x) { asm volatile("" : "+v"(x)); }
 // two values of bfloat16, zeros in the place of those that are not finite
 __device__ __forceinline__ uint32_t only_finite(uint32_t x) {
@@ -62,14 +69,17 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
     constexpr int KFR = 2 * KS, KC = KFR / 4, VC = DT / 4, CPI = KC + VC;      // fragments of a slice's keys, a wave's copies a step
     constexpr unsigned K_SLOT = KFR * 1024u, V_SLOT = DT * 1024u, V_BASE = NR * K_SLOT;
     constexpr int NPV = (DT + 1) * CT, NQK = KFR * CT, NS = NPV + NQK;         // a step's MFMAs (the sums' among them)
-    constexpr int NP = 4 * CT, FROM = 4, ITEMS = 3 * NP;                       // pairs of scores a lane, three instructions' worth each
+    constexpr int NP = 4 * CT, ITEMS = 3 * NP;                       // pairs of scores a lane, three instructions' worth each
     constexpr float LAG = 8.f;
     __shared__ __attribute__((aligned(1024))) char smem[V_BASE + NR * V_SLOT];
     __shared__ int32_t pages[TREE_PAGES];
     __shared__ uint32_t see[COLS * (TREE_WORDS + 1)];                          // the columns' bits, and a word of zeros
     __shared__ int first_seen[COLS];                                           // the first cached place of each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), qc = lane & 15, kg = lane >> 4;
-    const int g = blockIdx.x % a.nkv, b = blockIdx.x / a.nkv, G = a.nq / a.nkv;
+    const int G = a.nq / a.nkv;
+    int b, g;
+    tree_place(a.nkv, b, g);
+    if (b >= a.blocks) return;
     const bf16_t* __restrict__ kc = (const bf16_t*)a.k_cache + (size_t)g * a.page_size * D;
     const bf16_t* __restrict__ vc = (const bf16_t*)a.v_cache + (size_t)g * a.page_size * D;
     const size_t page_bytes = (size_t)a.nkv * a.page_size * D * 2;
@@ -102,52 +112,52 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
         const int s1 = min(t.slices, s0 + (u1 - u)), ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
 
-        // the columns: queries, bits, the first cached place of each
+        // The first chunk's page numbers, the columns' bits and the queries are asked for together.  (A chunk: slices whose page numbers fit,
+        // beginning anywhere in a page.)
+        const int last_block = (max(t.end, 1) - 1) & ~7;     // blocks of eight places lie in one page
+        const int chunk = max(1, ((TREE_PAGES - 2) << a.page_shift) >> 5);
+        auto chunk_page = [&](int c0) INLINE { return (t.first + c0 * 32) >> a.page_shift; };
+        auto chunk_pages = [&](int c0) INLINE {
+            return (min(last_block, t.first + min(c0 + chunk, s1) * 32 - 8) >> a.page_shift) - chunk_page(c0) + 1;
+        };
+        const int first_page = bt[chunk_page(s0) + min(tid, chunk_pages(s0) - 1)];
+        static_assert(COLS <= 256, "a thread a column");
+        const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + (min(tid & (COLS - 1), ncols - 1) + group * COLS) / G) * a.words, a.words,
+                                     t.end - t.start, t.start, a.window);
         bf16x8 q[CT][KS];
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             const int c = min((wave * CT + ct) * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
             const bf16_t* qp = (const bf16_t*)a.q + (size_t)(t.n0 + node) * a.q_stride + (size_t)head * D + kg * 8;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                uint4 x = *reinterpret_cast<const uint4*>(qp + ks * 32);
-                x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                q[ct][ks] = __builtin_bit_cast(bf16x8, x);
-            }
+            for (int ks = 0; ks < KS; ++ks) q[ct][ks] = *reinterpret_cast<const bf16x8*>(qp + ks * 32);
         }
         __syncthreads();                 // (the run before is done with LDS)
-        for (int c = tid; c < COLS; c += 256) {
-            const int node = (min(c, ncols - 1) + group * COLS) / G;
-            const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + node) * a.words, a.words, t.end - t.start, t.start, a.window);
+        if (tid < COLS) {
 #pragma unroll
-            for (int w = 0; w < TREE_WORDS; ++w) see[c * (TREE_WORDS + 1) + w] = row.bits[w];
-            see[c * (TREE_WORDS + 1) + TREE_WORDS] = 0;
-            first_seen[c] = row.lo;
+            for (int w = 0; w < TREE_WORDS; ++w) see[tid * (TREE_WORDS + 1) + w] = row.bits[w];
+            see[tid * (TREE_WORDS + 1) + TREE_WORDS] = 0;
+            first_seen[tid] = row.lo;
         }
 
         floatx4 o[CT][DT + 1], sc[2][CT][2];         // (the last of o: the sums, four times the same)
         bf16x8 pf[2][CT], kf[KFR], vf[DT], ones;
-        float top_ref[CT], neg_ref[CT], factor[CT];  // a column's reference, minus the same in the exponent's units, what its outputs still want
+        float top_ref[CT], limit[CT], neg_ref[CT], factor[CT];  // a column's reference, what a score may be, minus the reference in the exponent's units, what the outputs still want
         bool rescale = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ones[i] = (bf16_t)1.f;
         hold(ones);                      // (in registers from here on: made anew right before an MFMA, which the compiler does not know for one, they came too late)
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
-            top_ref[ct] = -INFINITY;
+            top_ref[ct] = limit[ct] = -INFINITY;
             neg_ref[ct] = 0.f;
             factor[ct] = 1.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+a"(q[ct][ks]));
         }
         each<CT * (DT + 1)>([&](auto I) INLINE {
             floatx4& x = o[decltype(I)::value % CT][decltype(I)::value / CT];
             x = floatx4{0.f, 0.f, 0.f, 0.f};
             pin(x);
         });
-        const int last_block = (max(t.end, 1) - 1) & ~7;     // blocks of eight places lie in one page
-        // slices of a chunk whose page numbers fit (a chunk begins anywhere in a page)
-        const int chunk = max(1, ((TREE_PAGES - 2) << a.page_shift) >> 5);
         int lo_most = 0, lo_least = 0;
 
         // which of the places key, key + 1, ... a column sees: a bit each (the next 8 of them hold)
@@ -162,7 +172,6 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
             return (((1u << cached) - 1) & (~0u << below)) | (-j < 32 ? row[0] << -j : 0u);
         };
         auto settle = [&](floatx4 (&x)[CT][2]) INLINE {
-            asm volatile("s_nop 15");
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) asm volatile("" : "+v"(x[ct][0]), "+v"(x[ct][1]));
         };
@@ -285,10 +294,10 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                 __syncthreads();
             }
             // (slices past the chunk's end are copied ahead in vain: their places are held to its pages)
-            page0 = (t.first + c0 * 32) >> a.page_shift;
-            const int end_block = min(last_block, t.first + (c0 + n) * 32 - 8);
-            for (int i = tid; i <= (end_block >> a.page_shift) - page0; i += 256) {
-                const int p = bt[page0 + i];
+            page0 = chunk_page(c0);
+            const int pages_n = chunk_pages(c0);
+            for (int i = tid; i < pages_n; i += 256) {
+                const int p = c0 == s0 && i == tid ? first_page : bt[page0 + i];
                 pages[i] = (unsigned)p < (unsigned)a.num_pages ? p : 0;
             }
             __syncthreads();
@@ -317,6 +326,17 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                     unsigned long long va = v_at(held(x - 1));
                     each<VC>([&](auto C) INLINE { copy_v(C, va, v_to + (x - 1) * V_SLOT); });
                 }
+            }
+            if (c0 == s0) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        uint4 x = __builtin_bit_cast(uint4, q[ct][ks]);
+                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                        q[ct][ks] = __builtin_bit_cast(bf16x8, x);
+                        to_acc(q[ct][ks]);
+                    }
             }
             __builtin_amdgcn_s_waitcnt(vmcnt_imm((NR - 1) * CPI));
             __syncthreads();
@@ -370,7 +390,7 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                         if constexpr (NPV + dt * NQK / DT == n_) vf[dt] = *reinterpret_cast<const bf16x8*>(vsrc + dt * 1024);
                     });
                     // the softmax of slice s
-                    if constexpr (n_ == 2) {
+                    if constexpr (n_ == 4) {
                         if constexpr (CAP) cap(sc[h]);
                         if (is_masked(k0)) mask(sc[h], k0);
                         float top[CT];
@@ -378,24 +398,25 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
 #pragma unroll
                         for (int ct = 0; ct < CT; ++ct) {
                             const floatx4 &x = sc[h][ct][0], &y = sc[h][ct][1];
-                            top[ct] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-                            ahead |= top[ct] > top_ref[ct] + lag;
+                            top[ct] = largest3(largest3(x[0], x[1], x[2]), largest3(x[3], y[0], y[1]), largest3(y[2], y[3], y[3]));
+                            ahead |= top[ct] > limit[ct];
                         }
                         if (__any(ahead)) {
                             rescale = true;
 #pragma unroll
                             for (int ct = 0; ct < CT; ++ct) {
                                 const float m = rows_max(top[ct]);
-                                const bool up = m > top_ref[ct] + lag;
+                                const bool up = m > limit[ct];
                                 factor[ct] = up ? __builtin_amdgcn_exp2f((top_ref[ct] - m) * sl2) : 1.f;
                                 top_ref[ct] = up ? m : top_ref[ct];
+                                limit[ct] = up ? m + lag : limit[ct];
                                 neg_ref[ct] = top_ref[ct] == -INFINITY ? 0.f : -top_ref[ct] * sl2;
-                                asm volatile("" : "+v"(factor[ct]), "+v"(top_ref[ct]), "+v"(neg_ref[ct]));
+                                asm volatile("" : "+v"(factor[ct]), "+v"(top_ref[ct]), "+v"(neg_ref[ct]), "+v"(limit[ct]));
                             }
                         }
                     }
-                    if constexpr (n_ > 2) {
-                        constexpr int i0 = (n_ - 3) * ITEMS / (NS - 3), i1 = (n_ - 2) * ITEMS / (NS - 3);
+                    if constexpr (n_ > 4) {
+                        constexpr int i0 = (n_ - 5) * ITEMS / (NS - 5), i1 = (n_ - 4) * ITEMS / (NS - 5);
                         each<i1 - i0>([&](auto I) INLINE {
                             constexpr int i = i0 + decltype(I)::value, p = i / 3, ct = p / 4, e = (p % 4) * 2;
                             if constexpr (i % 3 == 0) {
@@ -510,7 +531,7 @@ int tree_wide_tiles(int columns, int d) {
 int tree_wide_blocks_per_cu(int d, int tiles) { return blocks_of(d, tiles); }
 
 int tree_wide_launch(const TreeArgs& a, int d, int tiles, hipStream_t stream) {
-    const int grid = a.nkv * a.blocks;
+    const int grid = tree_grid(a.nkv, a.blocks);
 #define TFF_TREE_W(D, CT)                                                                       \
     do {                                                                                        \
         if (a.softcap > 0.f) tree_wide_kernel<D, CT, true><<<grid, 256, 0, stream>>>(a);        \

@@ -13,8 +13,10 @@ with a device dispatch; here the table has one entry per op and no dispatch.
 from __future__ import annotations
 
 import ctypes
+import functools
 import heapq
 import math
+import operator
 
 import numpy as np
 import torch
@@ -2605,22 +2607,30 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, uniform: torch.Tenso
 
 # ---- options on logits, trees of drafted tokens ----
 
-def _int_row(t, name: str, n: int | None = None) -> int:
-    """The address of an int32 tensor of one dimension, of n elements where n is given."""
-    _req(t, name, torch.int32, 1)
-    if n is not None and t.numel() != n:
-        raise _lib.KernelError(f"{name}: {t.numel()} elements, expected {n}")
+def _place(t: torch.Tensor, what: str) -> int:
+    """The number of the GPU that a call's first operand is on, which has to be the current one: a launch goes to its stream."""
+    dev = torch.cuda.current_device() if isinstance(t, torch.Tensor) and t.is_cuda else -1
+    if dev < 0:
+        raise _lib.KernelError(f"{what}: expected a tensor on the GPU")
+    if t.get_device() != dev:
+        raise _lib.KernelError(f"{what}: the operands are on {t.device}, the current device is cuda:{dev}")
+    return dev
+
+
+def _operand(t: torch.Tensor, dev: int, dtype: torch.dtype, ndim: int, what: str, name: str, n: int = -1) -> int:
+    """The address of a contiguous tensor of this type and so many dimensions on GPU ``dev`` (and of n elements).  One line of tests: the
+    calls that use it take some microseconds, most of them here."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype is not dtype or t.dim() != ndim or not t.is_contiguous() \
+            or (n >= 0 and t.numel() != n):
+        _req(t, f"{what} {name}", dtype, ndim)
+        if t.get_device() != dev:
+            raise _lib.KernelError(f"{what} {name}: on {t.device}, other operands on cuda:{dev}")
+        raise _lib.KernelError(f"{what} {name}: {t.numel()} elements, expected {n}")
     return t.data_ptr()
 
 
-def _one_device(what: str, device, *tensors) -> None:
-    """Operands on one device, which is the current one: a launch goes to the current device's stream."""
-    if device.index != torch.cuda.current_device():
-        raise _lib.KernelError(f"{what}: the operands are on {device}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise _lib.KernelError(f"{what}: operands on {device} and on {t.device}")
-
+_dtype_of, _shape_of = operator.attrgetter("dtype"), operator.attrgetter("shape")
+_gpu_of, _contiguous, _address = torch.Tensor.get_device, torch.Tensor.is_contiguous, torch.Tensor.data_ptr
 
 #: words of 32 bits that a row of a tree's ancestors has at most
 TREE_WORDS = 8
@@ -2628,11 +2638,11 @@ TREE_WORDS = 8
 TREE_PATH = 32 * TREE_WORDS
 
 
-def _ancestors(t, what: str, rows: int) -> int:
-    _req(t, what + " ancestors", torch.int32, 2)
+def _ancestors(t, dev: int, what: str, rows: int) -> int:
+    at = _operand(t, dev, torch.int32, 2, what, "ancestors")
     if t.shape[0] != rows or not 0 < t.shape[1] <= TREE_WORDS:
         raise _lib.KernelError(f"{what}: ancestors {tuple(t.shape)} are not [{rows}, 1 .. {TREE_WORDS}]")
-    return t.shape[1]
+    return at
 
 
 def adjust_logits(logits: torch.Tensor, history: torch.Tensor, cu_history: torch.Tensor, prompt_lens: torch.Tensor,
@@ -2647,56 +2657,53 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, cu_history: torch
     int32 [rows]): the tokens a row may choose, a bit each (lowest first), and the row's mask (-1: none); the others get -inf.
     ``drafts`` = (int32 tokens [rows], int32 cu_nodes [requests + 1], int32 ancestors [rows, words]): the rows are nodes of drafted trees
     (:func:`tree_attention`) and have the tokens of the nodes they see as output, too; without it row i is request i's."""
-    _req(logits, "adjust_logits logits", torch.float32, 2)
+    what, i32, f32 = "adjust_logits", torch.int32, torch.float32
+    dev = _place(logits, what)
+    x = _operand(logits, dev, f32, 2, what, "logits")
     rows, V = logits.shape
+    cu = _operand(cu_history, dev, i32, 1, what, "cu_history")
     requests = cu_history.numel() - 1
     if requests < 0:
         raise _lib.KernelError("adjust_logits: cu_history has no elements")
-    _int_row(history, "adjust_logits history")
-    _int_row(cu_history, "adjust_logits cu_history")
-    _int_row(prompt_lens, "adjust_logits prompt_lens", requests)
-    for t, name in ((repetition, "repetition"), (presence, "presence"), (frequency, "frequency")):
-        _req(t, name, torch.float32, 1)
-        if t.numel() != requests:
-            raise _lib.KernelError(f"adjust_logits: {t.numel()} numbers of {name} for {requests} requests")
-    ids = values = cu_bias = mask_bits = mask_rows = tokens = cu_nodes = ancestors = None
-    words = 0
+    ids = values = cu_bias = bits = mask_rows = tokens = cu_nodes = ancestors = None
+    num_bias = num_masks = words = 0
     if bias is not None:
-        ids, values, cu_bias = bias
-        _int_row(ids, "adjust_logits bias ids")
-        _int_row(cu_bias, "adjust_logits cu_bias", requests + 1)
-        _req(values, "adjust_logits bias values", torch.float32, 1)
-        if values.numel() != ids.numel():
-            raise _lib.KernelError(f"adjust_logits: {values.numel()} biases for {ids.numel()} tokens")
+        values = _operand(bias[1], dev, f32, 1, what, "bias values")
+        num_bias = bias[1].numel()
+        ids = _operand(bias[0], dev, i32, 1, what, "bias ids", num_bias)
+        cu_bias = _operand(bias[2], dev, i32, 1, what, "cu_bias", requests + 1)
     if masks is not None:
-        mask_bits, mask_rows = masks
-        _req(mask_bits, "adjust_logits masks", torch.int32, 2)
-        if mask_bits.shape[1] != -(-V // 32):
-            raise _lib.KernelError(f"adjust_logits: masks of {mask_bits.shape[1]} words for {V} tokens")
-        _int_row(mask_rows, "adjust_logits mask rows", rows)
+        bits = _operand(masks[0], dev, i32, 2, what, "masks")
+        num_masks = masks[0].shape[0]
+        if masks[0].shape[1] != -(-V // 32):
+            raise _lib.KernelError(f"adjust_logits: masks of {masks[0].shape[1]} words for {V} tokens")
+        mask_rows = _operand(masks[1], dev, i32, 1, what, "mask rows", rows)
     if drafts is not None:
-        tokens, cu_nodes, ancestors = drafts
-        _int_row(tokens, "adjust_logits draft tokens", rows)
-        _int_row(cu_nodes, "adjust_logits cu_nodes", requests + 1)
-        words = _ancestors(ancestors, "adjust_logits", rows)
+        tokens = _operand(drafts[0], dev, i32, 1, what, "draft tokens", rows)
+        cu_nodes = _operand(drafts[1], dev, i32, 1, what, "cu_nodes", requests + 1)
+        ancestors = _ancestors(drafts[2], dev, what, rows)
+        words = drafts[2].shape[1]
     elif rows != requests:
         raise _lib.KernelError(f"adjust_logits: {rows} rows of {requests} requests")
     if out is None:
         out = torch.empty_like(logits)
     elif out is not logits:
-        _req(out, "adjust_logits out", torch.float32, 2)
+        at = _operand(out, dev, f32, 2, what, "out")
         if out.shape != logits.shape:
             raise _lib.KernelError(f"adjust_logits out: shape {tuple(out.shape)} is not {(rows, V)}")
-        if out.data_ptr() != logits.data_ptr() and abs(out.data_ptr() - logits.data_ptr()) < 4 * rows * V:
+        if at != x and abs(at - x) < 4 * rows * V:
             raise _lib.KernelError("adjust_logits out: overlaps the logits without being them")
-    _one_device("adjust_logits", logits.device, history, cu_history, prompt_lens, repetition, presence, frequency, ids, values, cu_bias,
-                mask_bits, mask_rows, tokens, cu_nodes, ancestors, out)
     _lib.check(_lib.load().tff_adjust_logits(
-        logits.data_ptr(), out.data_ptr(), rows, V, requests, history.data_ptr(), history.numel(), cu_history.data_ptr(),
-        prompt_lens.data_ptr(), repetition.data_ptr(), presence.data_ptr(), frequency.data_ptr(), _ptr(ids), _ptr(values),
-        0 if ids is None else ids.numel(), _ptr(cu_bias), _ptr(mask_bits), 0 if mask_bits is None else mask_bits.shape[0], _ptr(mask_rows),
-        _ptr(tokens), _ptr(cu_nodes), _ptr(ancestors), words, _stream()))
+        x, out.data_ptr(), rows, V, requests, _operand(history, dev, i32, 1, what, "history"), history.numel(), cu,
+        _operand(prompt_lens, dev, i32, 1, what, "prompt_lens", requests), _operand(repetition, dev, f32, 1, what, "repetition", requests),
+        _operand(presence, dev, f32, 1, what, "presence", requests), _operand(frequency, dev, f32, 1, what, "frequency", requests), ids, values,
+        num_bias, cu_bias, bits, num_masks, mask_rows, tokens, cu_nodes, ancestors, words, _stream()))
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(rows: int, R: int, nq: int, nkv: int, d: int, page_size: int, width: int, code: int, dev: int) -> int:
+    return _lib.load().tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, page_size, width, code)
 
 
 def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -2710,38 +2717,38 @@ def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Te
     see :func:`paged_attention`.  Returns [rows, nq * d] in q's type, which is the cache's; a node that sees nothing gets zeros, rows that
     no request has are left as they are.  Up to 256 nodes a request, head sizes up to 512; a token's bits may depend on what else is in the
     step, as they do where decoding splits keys.  The table of pages has to reach to a request's last node."""
-    _req(q, "tree_attention q", ndim=2)
-    rows = q.shape[0]
-    if q.shape[1] < nq * d:
-        raise _lib.KernelError(f"tree_attention q: rows of {q.shape[1]} hold fewer than nq*d = {nq * d}")
-    _req(k_cache, "k cache", q.dtype, 4)
-    _req(v_cache, "v cache", q.dtype, 4)
-    _check_cache(k_cache, v_cache, nkv, d, "tree_attention")
-    _req(block_tables, "block tables", torch.int32, 2)
+    what, i32 = "tree_attention", torch.int32
+    dev = _place(q, what)
+    dtype = q.dtype
+    qp = _operand(q, dev, dtype, 2, what, "q")
+    rows, width = q.shape
+    if width < nq * d:
+        raise _lib.KernelError(f"tree_attention q: rows of {width} hold fewer than nq*d = {nq * d}")
+    kp, vp = _operand(k_cache, dev, dtype, 4, what, "k cache"), _operand(v_cache, dev, dtype, 4, what, "v cache")
+    _check_cache(k_cache, v_cache, nkv, d, what)
+    pages, _, page_size, _ = k_cache.shape
+    table = _operand(block_tables, dev, i32, 2, what, "block tables")
+    start = _operand(start_pos, dev, i32, 1, what, "start_pos")
     R = start_pos.numel()
-    _int_row(start_pos, "tree_attention start_pos")
-    _int_row(cu_nodes, "tree_attention cu_nodes", R + 1)
+    cu = _operand(cu_nodes, dev, i32, 1, what, "cu_nodes", R + 1)
     if block_tables.shape[0] != R:
         raise _lib.KernelError(f"tree_attention: tables of {block_tables.shape[0]} requests for {R}")
-    words = _ancestors(ancestors, "tree_attention", rows)
-    _check_sinks(sinks, nq)
+    bits = _ancestors(ancestors, dev, what, rows)
+    sink = None if sinks is None else _operand(sinks, dev, torch.float32, 1, what, "sinks", nq)
     if out is None:
-        out = torch.empty(rows, nq * d, dtype=q.dtype, device=q.device)
+        out = torch.empty(rows, nq * d, dtype=dtype, device=q.device)
     else:
-        _req(out, "tree_attention out", q.dtype, 2)
+        _operand(out, dev, dtype, 2, what, "out")
         if tuple(out.shape) != (rows, nq * d):
             raise _lib.KernelError(f"tree_attention out: shape {tuple(out.shape)} is not {(rows, nq * d)}")
-    _one_device("tree_attention", q.device, k_cache, v_cache, block_tables, cu_nodes, start_pos, ancestors, sinks, out)
     if scale is None:
         scale = 1.0 / math.sqrt(d)
-    L, code = _lib.load(), dtype_code(q.dtype)
-    room = L.tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, k_cache.shape[2], block_tables.stride(0), code)
-    ws = torch.empty(room // 4, dtype=torch.float32, device=q.device) if room else None
+    L, code, tables_width = _lib.load(), dtype_code(dtype), block_tables.shape[1]
+    room = _tree_workspace(rows, R, nq, nkv, d, page_size, tables_width, code, dev)
+    ws = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
     _lib.check(L.tff_tree_attention(
-        q.data_ptr(), q.stride(0), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-        block_tables.stride(0), cu_nodes.data_ptr(), start_pos.data_ptr(), ancestors.data_ptr(), words, R, rows, nq, nkv, d,
-        k_cache.shape[2], k_cache.shape[0], int(window), float(scale), _ptr(sinks), float(softcap or 0.0), _ptr(ws), room,
-        code, _stream()))
+        qp, width, out.data_ptr(), kp, vp, table, tables_width, cu, start, bits, ancestors.shape[1], R, rows, nq, nkv, d, page_size, pages,
+        int(window), float(scale), sink, float(softcap or 0.0), _ptr(ws), room, code, _stream()))
     return out
 
 
@@ -2750,20 +2757,23 @@ def tree_accept(choices: torch.Tensor, tokens: torch.Tensor, cu_nodes: torch.Ten
     whose token is what the model chose after its parent (``choices``, ``tokens``: int32 [rows]).  Returns int32 ``path``
     [requests, max_path] (the kept nodes' numbers in their tree, then -1), ``counts`` [requests] and ``next`` [requests], the choice after
     the last kept node; a request without nodes gets 0 and -1.  A path ends at ``max_path`` nodes."""
-    T, R = tokens.numel(), cu_nodes.numel() - 1
-    _int_row(tokens, "tree_accept tokens")
-    _int_row(choices, "tree_accept choices", T)
-    _int_row(cu_nodes, "tree_accept cu_nodes")
+    what, i32 = "tree_accept", torch.int32
+    dev = _place(tokens, what)
+    t = _operand(tokens, dev, i32, 1, what, "tokens")
+    T = tokens.numel()
+    c = _operand(choices, dev, i32, 1, what, "choices", T)
+    cu = _operand(cu_nodes, dev, i32, 1, what, "cu_nodes")
+    R = cu_nodes.numel() - 1
     if R < 0:
         raise _lib.KernelError("tree_accept: cu_nodes has no elements")
-    words = _ancestors(ancestors, "tree_accept", T)
+    bits = _ancestors(ancestors, dev, what, T)
     if not 0 < max_path <= TREE_PATH:
         raise _lib.KernelError(f"tree_accept: paths of {max_path} nodes (1 .. {TREE_PATH})")
-    _one_device("tree_accept", tokens.device, choices, cu_nodes, ancestors)
-    made = torch.empty(R * (max_path + 2), dtype=torch.int32, device=tokens.device)
-    path, counts, following = made[:R * max_path].view(R, max_path), made[R * max_path:R * (max_path + 1)], made[R * (max_path + 1):]
-    _lib.check(_lib.load().tff_tree_accept(choices.data_ptr(), tokens.data_ptr(), cu_nodes.data_ptr(), ancestors.data_ptr(), words, T, R,
-                                           int(max_path), path.data_ptr(), counts.data_ptr(), following.data_ptr(), _stream()))
+    path = torch.empty(R, max_path, dtype=i32, device=tokens.device)
+    rest = torch.empty(2, R, dtype=i32, device=tokens.device)
+    at = rest.data_ptr()
+    _lib.check(_lib.load().tff_tree_accept(c, t, cu, bits, ancestors.shape[1], T, R, int(max_path), path.data_ptr(), at, at + 4 * R, _stream()))
+    counts, following = rest.unbind(0)
     return path, counts, following
 
 
@@ -2772,36 +2782,38 @@ def cache_keep(caches: list, block_tables: torch.Tensor, start_pos: torch.Tensor
     (keys, values) of one shape, as the layers of a group have them) at once: for i < counts[r], place ``start_pos[r] + path[r, i]`` of
     request r's pages to place ``start_pos[r] + i``.  ``path`` int32 [requests, up to 256] and ``counts`` as :func:`tree_accept` returns
     them.  Two requests must not share the pages that their nodes lie in."""
+    what, i32 = "cache_keep", torch.int32
+    dev = _place(start_pos, what)
+    start = _operand(start_pos, dev, i32, 1, what, "start_pos")
     R = start_pos.numel()
-    _int_row(start_pos, "cache_keep start_pos")
-    _int_row(counts, "cache_keep counts", R)
-    _req(path, "cache_keep path", torch.int32, 2)
-    _req(block_tables, "block tables", torch.int32, 2)
+    kept = _operand(counts, dev, i32, 1, what, "counts", R)
+    places = _operand(path, dev, i32, 2, what, "path")
+    table = _operand(block_tables, dev, i32, 2, what, "block tables")
     if path.shape[0] != R or block_tables.shape[0] != R or not 0 < path.shape[1] <= TREE_PATH:
         raise _lib.KernelError(f"cache_keep: paths {tuple(path.shape)} and tables {tuple(block_tables.shape)} for {R} requests")
     if not caches:
         return
-    shape, dtype, device = caches[0][0].shape, caches[0][0].dtype, caches[0][0].device
-    if len(shape) != 4:
-        raise _lib.KernelError(f"k cache: expected 4 dimensions, got shape {tuple(shape)}")
-    pages, nkv, page_size, d = shape
-    vshape, keys, values = (pages, nkv, d, page_size), [], []
-    for k, v in caches:
-        if k.shape != shape or v.shape != vshape or k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device \
-                or not k.is_contiguous() or not v.is_contiguous():
-            raise _lib.KernelError(f"cache_keep: caches {tuple(k.shape)} / {tuple(v.shape)} of {k.dtype} beside {tuple(shape)} of {dtype}")
-        keys.append(k.data_ptr())
-        values.append(v.data_ptr())
-    if not caches[0][0].is_cuda:
-        raise _lib.KernelError("cache_keep: expected a tensor on the GPU")
-    _one_device("cache_keep", device, block_tables, start_pos, path, counts)
-    n = len(keys)
-    if len(set(keys)) != n or len(set(values)) != n:
+    keys, values = zip(*caches)
+    first, n = keys[0], len(keys)
+    _operand(first, dev, first.dtype, 4, what, "k cache")
+    pages, nkv, page_size, d = first.shape
+    # (the layers' caches at once: dozens of tensors, and a test of one of them by itself takes as long as the kernel)
+    both = keys + values
+    if set(map(_dtype_of, both)) != {first.dtype} or set(map(_shape_of, keys)) != {first.shape} or set(map(_gpu_of, both)) != {dev} \
+            or set(map(_shape_of, values)) != {(pages, nkv, d, page_size)} or not all(map(_contiguous, both)):
+        for k, v in caches:
+            _operand(k, dev, first.dtype, 4, what, "k cache")
+            _operand(v, dev, first.dtype, 4, what, "v cache")
+            if k.shape != first.shape:
+                raise _lib.KernelError(f"cache_keep: keys {tuple(k.shape)} beside {tuple(first.shape)}")
+            _check_cache(k, v, nkv, d, what)
+    at = list(map(_address, both))
+    if len(set(at)) != 2 * n:
         raise _lib.KernelError("cache_keep: a cache is listed twice")
-    kp, vp = (ctypes.c_void_p * n)(*keys), (ctypes.c_void_p * n)(*values)
-    _lib.check(_lib.load().tff_cache_keep(
-        ctypes.addressof(kp), ctypes.addressof(vp), n, block_tables.data_ptr(), block_tables.stride(0), start_pos.data_ptr(), path.data_ptr(),
-        counts.data_ptr(), R, path.shape[1], nkv, d, page_size, pages, dtype_code(dtype), _stream()))
+    ptrs = (ctypes.c_void_p * (2 * n))(*at)
+    base = ctypes.addressof(ptrs)
+    _lib.check(_lib.load().tff_cache_keep(base, base + 8 * n, n, table, block_tables.shape[1], start, places, kept, R, path.shape[1], nkv, d,
+                                          page_size, pages, dtype_code(first.dtype), _stream()))
 
 
 def measure_ceilings(device="cuda:0", gib: float = 4.0, quick: bool = False) -> dict:
