@@ -1,0 +1,103 @@
+"""Penalties, biases and grammars through the engine, beside requests that have none."""
+import numpy as np
+import pytest
+import torch
+
+import plain_draft_trees as plain
+from helpers import random_tokens
+from tffinfer_amd import EngineOptions, LLMEngine, SamplingConfig
+
+pytestmark = pytest.mark.gpu
+
+
+def packed(tokens, V):
+    return plain.packed([tokens], -(-V // 32))[0].numpy()
+
+
+def check_greedy(r, c, V, allowed=None):
+    """Every token is the first maximum of the kept logits after the options, in float32 as the kernel rounds; where float64 finds two candidates
+    closer than the rounding of a few operations (2^-20 of their size) either will do."""
+    for i, (row, tok) in enumerate(zip(r.logits, r.output)):
+        f = lambda x: float(torch.tensor(x, dtype=torch.float32))  # noqa: E731
+        masks = None if allowed is None else [allowed(r.output[:i])]
+        x, _ = plain.adjust(row.view(1, V).float(), [r.prompt + r.output[:i]], [len(r.prompt)], [f(c.repetition_penalty)], [f(c.presence_penalty)],
+                            [f(c.frequency_penalty)], [[(t, f(b)) for t, b in (c.logit_bias or {}).items()]], masks,
+                            None if masks is None else [0 if masks[0] is not None else -1])
+        best = float(x.max())
+        assert float(x[0, tok]) >= best - 2.0 ** -20 * max(1.0, abs(best)), (i, tok)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_options_through_the_engine(model_dirs, dtype, graphs):
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype=dtype, kv_tokens=512, max_num_seqs=6, use_graphs=graphs))
+    eng.keep_logits = True
+    V = eng.model.config.vocab_size
+    prompts = [random_tokens(n, V, 40 + n) for n in (4, 9, 17, 5, 6, 30)]
+    even = list(range(0, V, 2))
+
+    def alternate(out):
+        return None if len(out) % 3 == 2 else (even if len(out) % 2 else list(range(1, V, 2)))
+    configs = [SamplingConfig(), SamplingConfig(presence_penalty=3.0, frequency_penalty=0.5), SamplingConfig(logit_bias={7: 50.0, 3: -100.0}),
+               SamplingConfig(repetition_penalty=1.7), SamplingConfig(allowed=lambda out: None if alternate(out) is None else packed(alternate(out), V)),
+               SamplingConfig(repetition_penalty=1.2, frequency_penalty=1.0, logit_bias={11: 2.0}, allowed=lambda out: packed(even, V))]
+    res = eng.generate(prompts, configs, max_new_tokens=20, ignore_eos=True)
+    for r, c, a in zip(res, configs, (None, None, None, None, alternate, lambda out: even)):
+        assert len(r.output) == 20
+        check_greedy(r, c, V, a)
+    assert set(res[2].output) == {7} and all(t % 2 == 0 for t in res[5].output)
+    assert len(set(res[1].output)) > len(set(eng.generate([prompts[1]], max_new_tokens=20, ignore_eos=True)[0].output)) - 1
+    # alone, and with the step ahead of a bias (which needs no output), the same tokens in float32
+    if dtype == "float32":
+        for p, c, r in zip(prompts, configs, res):
+            alone = LLMEngine(eng.model, EngineOptions(dtype=dtype, kv_tokens=256, max_num_seqs=1, use_graphs=graphs))
+            assert alone.generate([p], c, max_new_tokens=20, ignore_eos=True)[0].output == r.output
+            assert (alone.steps_ahead > 0) == (not c.needs_output)
+
+
+def test_a_draw_stays_within_the_grammar(model_dirs):
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="bfloat16", kv_tokens=256, max_num_seqs=3))
+    V = eng.model.config.vocab_size
+    few = [3, 40, V - 1]
+    c = [SamplingConfig("random", temperature=2.0, seed=s, allowed=lambda out: packed(few, V), frequency_penalty=0.5) for s in (1, 2, 3)]
+    for r in eng.generate([[1, 2], [5], [9, 9, 9]], c, max_new_tokens=24, ignore_eos=True):
+        assert set(r.output) <= set(few) and len(set(r.output)) > 1
+    none = eng.generate([[1, 2]], SamplingConfig(allowed=lambda out: np.zeros(-(-V // 32), dtype=np.int32)), max_new_tokens=3, ignore_eos=True)
+    assert none[0].output == [0, 0, 0]
+
+
+def test_a_grammar_that_fails_leaves_the_requests_where_they_stood(model_dirs):
+    d = model_dirs["A"]
+    eng = LLMEngine.from_model_dir(d, EngineOptions(dtype="float32", kv_tokens=256, max_num_seqs=2, page_size=8))
+    V = eng.model.config.vocab_size
+    fail = [False]
+
+    def grammar(out):
+        if fail[0]:
+            raise RuntimeError("no grammar")
+        return packed(range(0, V, 3), V)
+    prompts = [[1, 2, 3, 4, 5], [8, 9]]
+    configs = [SamplingConfig(allowed=grammar, repetition_penalty=1.3), SamplingConfig()]
+    want = [r.output for r in eng.generate(prompts, configs, max_new_tokens=20, ignore_eos=True)]
+    ids = [eng.add_request(p, c, 20, ignore_eos=True) for p, c in zip(prompts, configs)]
+    steps = 0
+    while eng.has_work:
+        steps += 1
+        if steps % 4 == 0:
+            fail[0] = True
+            with pytest.raises(RuntimeError, match="no grammar"):
+                eng.step()
+            fail[0] = False
+        eng.step()
+    assert [eng.pop_result(i).output for i in ids] == want
+    assert all(g.pool.num_used == 0 for g in eng.runner.cache.groups)
+
+
+def test_refusals(model_dirs):
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="float32", kv_tokens=64, max_num_seqs=1))
+    V = eng.model.config.vocab_size
+    with pytest.raises(ValueError, match="vocabulary"):
+        eng.add_request([1], SamplingConfig(logit_bias={V: 1.0}))
+    eng.add_request([1], SamplingConfig(allowed=lambda out: np.zeros(3, dtype=np.float32)))
+    with pytest.raises(ValueError, match="allowed"):
+        eng.step()

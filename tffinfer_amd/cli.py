@@ -23,6 +23,13 @@ import time
 from . import log
 
 
+def _parse_bias(text: str) -> dict:
+    try:
+        return {int(t): float(b) for t, b in (x.split(":") for x in text.replace(",", " ").split())}
+    except ValueError:
+        raise argparse.ArgumentTypeError(f"{text!r} is no list of token:bias") from None
+
+
 def build_parser() -> argparse.ArgumentParser:
     ap = argparse.ArgumentParser(prog="tffinfer", description=__doc__,
                                  formatter_class=argparse.RawDescriptionHelpFormatter)
@@ -66,6 +73,9 @@ def build_parser() -> argparse.ArgumentParser:
     g.add_argument("--top-p", type=float, default=1.0)
     g.add_argument("--min-p", type=float, default=0.0)
     g.add_argument("--repetition-penalty", type=float, default=1.0)
+    g.add_argument("--presence-penalty", type=float, default=0.0, help="off the logits of tokens in the output")
+    g.add_argument("--frequency-penalty", type=float, default=0.0, help="off them as often as they stand there")
+    g.add_argument("--logit-bias", type=_parse_bias, default=None, metavar="ID:BIAS,...", help="added to single tokens' logits")
     g.add_argument("--seed", type=int, default=0, help="seed of random weights and random prompts")
     g.add_argument("--sample-seed", type=int, default=None, help="seed of the random draws (default: --seed)")
     g = ap.add_argument_group("engine")
@@ -186,7 +196,8 @@ def main(argv=None) -> int:
         stype = "random"   # sampling options without a type mean a random draw
     sample_seed = args.seed if args.sample_seed is None else args.sample_seed
     cfg._sampling_config = SamplingConfig(stype, args.temperature, args.top_k, args.top_p, args.min_p,
-                                          args.repetition_penalty, sample_seed)
+                                          args.repetition_penalty, sample_seed, args.presence_penalty, args.frequency_penalty,
+                                          args.logit_bias)
     rt = LLMInferRuntime()
     t0 = time.time()
     if args.config:

@@ -56,7 +56,8 @@ TFF_ENGINE_API void engine_destroy(tff_engine* e);
 TFF_ENGINE_API int engine_vocab_size(tff_engine* e);
 
 // params_json: max_new_tokens, eos_token_id, ignore_eos, sampling {type, temperature, top_k, top_p,
-// min_p, repetition_penalty, seed}; NULL or "" for greedy and 64 tokens.  Returns the request's id.
+// min_p, repetition_penalty, seed, presence_penalty, frequency_penalty, logit_bias: {token: number}};
+// NULL or "" for greedy and 64 tokens.  Returns the request's id.
 TFF_ENGINE_API int64_t engine_add_request(tff_engine* e, const int32_t* token_ids, int32_t n, const char* params_json);
 // Plans and runs one step (prompt portions beside decoded tokens, as the scheduler cuts them) and
 // writes its events, at most capacity of them; returns their number.  Events that did not fit are

@@ -14,7 +14,7 @@ import torch
 
 from ..kernels import staging as _staging
 from ..models import load_model
-from ..sampling import Sampler, SamplingConfig, SeenTokens
+from ..sampling import Sampler, SamplingConfig, SeenTokens, TokenLog, allowed_mask
 from .batch import StepEntry
 from .runner import ModelRunner
 from .scheduler import Request, Scheduler, SchedulerOptions
@@ -169,6 +169,9 @@ class LLMEngine:
                 raise ValueError(f"token id {t} is outside the vocabulary of {V}")
         if eos_token_id is None and not ignore_eos:
             eos_token_id = getattr(self.model.config, "eos_token_id", None)
+        for t in (sampling.logit_bias or ()) if sampling is not None else ():
+            if t >= V:
+                raise ValueError(f"logit_bias: token id {t} is outside the vocabulary of {V}")
         req = Request(rid, prompt, sampling or SamplingConfig(), int(max_new_tokens), eos_token_id, ignore_eos)
         if rid in self._requests and self._requests[rid].status != "finished":
             raise ValueError(f"request id {rid!r} is in use")
@@ -213,6 +216,17 @@ class LLMEngine:
             entries.append(StepEntry(p.request.id, toks, [p.count - 1] if p.samples else []))
             if p.samples:
                 rows.append(p.request)
+        histories = masks = None
+        if any(r.sampling.adjusts for r in rows):
+            histories = [self._history(r) if r.sampling.adjusts else None for r in rows]
+            try:
+                # (before the step: a grammar that fails leaves the requests where they stood)
+                masks = [None if h is None else allowed_mask(r.sampling, h[0][h[1]:].copy(), self.model.config.vocab_size)
+                         for r, h in zip(rows, histories)]
+            except BaseException:
+                for p in plan:
+                    self.runner.cache.rollback(p.request.id)
+                raise
         logits = self.runner.step(entries, token_source)
         if not rows:
             return _Launched(plan, rows, None, None, None)
@@ -227,7 +241,7 @@ class LLMEngine:
         if any(r.sampling.repetition_penalty != 1.0 for r in rows):
             seen = [self._seen_tokens(r) if r.sampling.repetition_penalty != 1.0 else None for r in rows]
         tokens = self.sampler.sample_on_device(
-            logits, [r.sampling for r in rows], [len(r.output) + ahead for r in rows], seen)
+            logits, [r.sampling for r in rows], [len(r.output) + ahead for r in rows], seen, histories, masks)
         host = torch.empty(len(rows), dtype=torch.int32, pin_memory=True)
         host.copy_(tokens, non_blocking=True)
         ready = torch.cuda.Event()
@@ -242,6 +256,14 @@ class LLMEngine:
         if tracker is None:
             tracker = req._seen_tokens = SeenTokens()
         return tracker.update(req.tokens)
+
+    @staticmethod
+    def _history(req):
+        """The request's prompt and output as an array, kept with the request, and the prompt's length."""
+        log = getattr(req, "_token_log", None)
+        if log is None:
+            log = req._token_log = TokenLog(req.prompt)
+        return log.update(req.output), log.prompt_len
 
     def _complete(self, st: _Launched) -> list[tuple]:
         """Reads the step's tokens and tells the scheduler.  Requests that ended
@@ -262,8 +284,8 @@ class LLMEngine:
     def _plan_ahead(self, st: _Launched):
         """The decode step after ``st``, planned without its tokens: every request
         of ``st`` that its length does not end goes on.  None when the step after
-        needs the scheduler (admissions, prompts, pages running out, a penalty on
-        seen tokens)."""
+        needs the scheduler (admissions, prompts, pages running out) or the tokens
+        (a penalty on seen ones, a grammar)."""
         if not self.options.run_ahead or not st.rows:
             return None
         sch = self.scheduler
@@ -274,7 +296,7 @@ class LLMEngine:
         plan = []
         for p in st.plan:
             req = p.request
-            if req.status != "running" or req.sampling.repetition_penalty != 1.0:
+            if req.status != "running" or req.sampling.needs_output:
                 return None
             n_out = len(req.output) + 1           # with the token in flight
             if n_out >= req.max_new_tokens or len(req.prompt) + n_out >= sch.max_model_len:

@@ -4,7 +4,11 @@ SamplingConfig (src/core/sampler/LLMSampler.h:55-63): ``_type``,
 ``_seed`` there, the same without the underscore here."""
 from __future__ import annotations
 
-from dataclasses import dataclass
+import math
+from dataclasses import dataclass, field
+from typing import Callable
+
+import numpy as np
 
 #: strategy names of the reference (src/core/sampler/LLMSampler.h:18-24)
 STRATEGIES = ("default", "unknown", "greedy", "random", "top_k", "top_p")
@@ -30,6 +34,10 @@ class SamplingConfig:
     min_p: float = 0.0
     repetition_penalty: float = 1.0
     seed: int = 0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict | None = None
+    allowed: Callable[[np.ndarray], np.ndarray | None] | None = field(default=None, compare=False)
 
     def __post_init__(self):
         if self.type not in STRATEGIES or self.type == "unknown":
@@ -40,6 +48,24 @@ class SamplingConfig:
             raise ValueError("top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1 are required")
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be positive")
+        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be numbers")
+        if self.allowed is not None and not callable(self.allowed):
+            raise ValueError("allowed must be a function of the output so far")
+        if self.logit_bias is not None:
+            self.logit_bias = {int(t): float(b) for t, b in self.logit_bias.items()}
+            if any(not b < math.inf for b in self.logit_bias.values()) or any(not 0 <= t < 1 << 31 for t in self.logit_bias):
+                raise ValueError("logit_bias: tokens must not be negative, biases numbers (or -inf, never again)")
+
+    @property
+    def adjusts(self) -> bool:
+        """Whether the logits are changed by more than a repetition penalty."""
+        return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed)
+
+    @property
+    def needs_output(self) -> bool:
+        """Whether a token's choice depends on the tokens before it other than through the model."""
+        return bool(self.repetition_penalty != 1.0 or self.presence_penalty or self.frequency_penalty or self.allowed)
 
     @property
     def greedy(self) -> bool:

@@ -51,6 +51,37 @@ class SeenTokens:
         return self._buf[:self._n]
 
 
+class TokenLog:
+    """A request's prompt and output as one int32 array, kept up to date token by token."""
+
+    def __init__(self, prompt):
+        self.prompt_len = len(prompt)
+        self._n = len(prompt)
+        self._buf = np.empty(2 * self._n + 256, dtype=np.int32)
+        self._buf[:self._n] = prompt
+
+    def update(self, output) -> np.ndarray:
+        """``output``: the output so far, longer than (or as long as) at the last call."""
+        end = self.prompt_len + len(output)
+        if end > self._buf.size:
+            self._buf = np.concatenate([self._buf, np.empty(max(self._buf.size, end - self._buf.size), dtype=np.int32)])
+        if end > self._n:
+            self._buf[self._n:end] = output[self._n - self.prompt_len:]
+            self._n = end
+        return self._buf[:end]
+
+
+def allowed_mask(config: SamplingConfig, output: np.ndarray, vocab: int) -> np.ndarray | None:
+    """What the config's ``allowed`` says about the token after ``output``: int32 [ceil(vocab / 32)], or None for all."""
+    mask = config.allowed(output) if config.allowed is not None else None
+    if mask is None:
+        return None
+    mask = np.ascontiguousarray(mask)
+    if mask.dtype not in (np.int32, np.uint32) or mask.shape != (-(-vocab // 32),):
+        raise ValueError(f"allowed() returned {mask.dtype} {mask.shape}, expected int32 or uint32 {(-(-vocab // 32),)}")
+    return mask.view(np.int32)
+
+
 class Sampler:
     def __init__(self, device, ops=_ops):
         self.device = device
@@ -62,23 +93,66 @@ class Sampler:
         return _staging.send(self.device, columns)
 
     def sample(self, logits: torch.Tensor, configs: list[SamplingConfig], indices: list[int],
-               seen: list | None = None) -> list[int]:
+               seen: list | None = None, histories: list | None = None, masks: list | None = None) -> list[int]:
         """One token per row.  ``indices[r]`` is the number of the output token
         row r decides (the counter of its random draw); ``seen[r]`` the tokens
         of its prompt and output so far (needed only with a repetition penalty):
         a sequence, or its distinct tokens as an int32 array (``SeenTokens``).
-        ``logits`` may be changed in place by the penalty."""
+        ``histories[r]`` is (prompt and output as an int32 array, tokens of the prompt), for rows whose
+        config says ``adjusts`` (``TokenLog``); ``masks[r]`` is ``allowed_mask`` of the row (asked for here where not given).
+        ``logits`` may be changed in place by the options."""
         if logits.shape[0] == 0:
             return []
-        return self.sample_on_device(logits, configs, indices, seen).tolist()
+        return self.sample_on_device(logits, configs, indices, seen, histories, masks).tolist()
+
+    def _adjust(self, logits: torch.Tensor, configs: list[SamplingConfig], seen, histories, given) -> None:
+        """All options on the logits in one launch, a repetition penalty among them."""
+        V = logits.shape[1]
+        parts, cu, prompt_lens, ids, values, cu_bias, masks, mask_rows = [], [0], [], [], [], [0], [], []
+        for r, c in enumerate(configs):
+            tokens, prompt_len, mask = np.zeros(0, dtype=np.int32), 0, None
+            if c.adjusts and c.needs_output:
+                if histories is None or histories[r] is None:
+                    raise ValueError(f"row {r}: its options need the request's prompt and output")
+                tokens, prompt_len = histories[r]
+                mask = allowed_mask(c, tokens[prompt_len:].copy(), V) if given is None else given[r]
+            elif c.repetition_penalty != 1.0 and seen is not None:      # (which tokens it saw is all that counts)
+                tokens = np.asarray(seen[r], dtype=np.int32)
+                prompt_len = tokens.size
+            if c.repetition_penalty == 1.0 and not (c.presence_penalty or c.frequency_penalty):
+                tokens = tokens[:0]                                      # (nothing to send)
+            parts.append(tokens)
+            cu.append(cu[-1] + tokens.size)
+            prompt_lens.append(min(prompt_len, tokens.size))
+            if c.logit_bias:
+                ids.extend(c.logit_bias)
+                values.extend(c.logit_bias.values())
+            cu_bias.append(len(ids))
+            if mask is None:
+                mask_rows.append(-1)
+            else:
+                mask_rows.append(len(masks))
+                masks.append(mask)
+        columns = [np.concatenate(parts) if cu[-1] else np.zeros(0, dtype=np.int32), np.asarray(cu, dtype=np.int32),
+                   np.asarray(prompt_lens, dtype=np.int32), np.asarray([c.repetition_penalty for c in configs], dtype=np.float32),
+                   np.asarray([c.presence_penalty for c in configs], dtype=np.float32),
+                   np.asarray([c.frequency_penalty for c in configs], dtype=np.float32)]
+        if ids:
+            columns += [np.asarray(ids, dtype=np.int32), np.asarray(values, dtype=np.float32), np.asarray(cu_bias, dtype=np.int32)]
+        if masks:
+            columns += [np.stack(masks), np.asarray(mask_rows, dtype=np.int32)]
+        sent = self._send(columns)
+        self.ops.adjust_logits(logits, *sent[:6], bias=tuple(sent[6:9]) if ids else None, masks=tuple(sent[-2:]) if masks else None, out=logits)
 
     def sample_on_device(self, logits: torch.Tensor, configs: list[SamplingConfig], indices: list[int],
-                         seen: list | None = None) -> torch.Tensor:
+                         seen: list | None = None, histories: list | None = None, masks: list | None = None) -> torch.Tensor:
         """As ``sample``, but the tokens stay on the device (int32 [rows]) and
         nothing waits for them: the caller reads them when it needs them."""
         R = logits.shape[0]
         assert len(configs) == R and len(indices) == R
-        if any(c.repetition_penalty != 1.0 for c in configs):
+        if any(c.adjusts for c in configs):
+            self._adjust(logits, configs, seen, histories, masks)
+        elif any(c.repetition_penalty != 1.0 for c in configs):
             parts, cu = [], [0]
             for r, c in enumerate(configs):
                 if c.repetition_penalty != 1.0 and seen is not None:
