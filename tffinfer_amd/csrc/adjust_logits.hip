@@ -56,7 +56,6 @@ template <int RUN>
 __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, const int vec) {
     constexpr int PER = RUN / 1024;
     __shared__ __attribute__((aligned(16))) uint32_t cnt[RUN];
-    __shared__ uint32_t touched[RUN / 32];       // which tokens have a count
     const int t = blockIdx.x / a.runs, v0 = (blockIdx.x - t * a.runs) * RUN, n = min(RUN, a.V - v0), tid = threadIdx.x;
     const size_t base = (size_t)t * a.V + v0;
     const float* x = a.logits + base;
@@ -68,13 +67,45 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     r = __builtin_amdgcn_readfirstlane(r);
     const bool has_request = r < a.requests;      // (a row behind the last node is left as it is)
     const int32_t* __restrict__ mask = has_request && mask_row >= 0 && mask_row < a.num_masks ? a.masks + (size_t)mask_row * a.mask_words : nullptr;
+    // (all that the rest hangs on, asked for at once)
     float rep = 1.f, pres = 0.f, freq = 0.f;
+    int h0 = 0, h1 = 0, out0 = 0, b0 = 0, b1 = 0;
     if (has_request) {
         rep = a.repetition[r];
         pres = a.presence[r];
         freq = a.frequency[r];
+        h0 = a.cu_history[r];
+        h1 = a.cu_history[r + 1];
+        out0 = a.prompt_lens[r];
+        if (a.cu_bias) {
+            b0 = a.cu_bias[r];
+            b1 = a.cu_bias[r + 1];
+        }
     }
-    const bool counts = rep != 1.f || pres != 0.f || freq != 0.f;
+    h0 = min(max(h0, 0), a.history_len);
+    h1 = min(max(h1, h0), a.history_len);
+    out0 = h0 + min(max(out0, 0), h1 - h0);
+    b0 = min(max(b0, 0), a.bias_len);
+    b1 = min(max(b1, b0), a.bias_len);
+    const bool counts = h0 < h1 || a.cu_nodes ? rep != 1.f || pres != 0.f || freq != 0.f : false;
+    const int q0 = min(h1, (h0 + 3) & ~3), q1 = max(q0, h1 & ~3);      // (the part of the history that int4 loads can take)
+    const bool hvec = ((uintptr_t)a.history & 15) == 0;
+    // the thread's first bias and the history's first tokens (a thread's share of the others is asked for three steps ahead)
+    int bias_id = -1;
+    float bias = 0.f;
+    if (b0 + tid < b1) {
+        bias_id = a.bias_ids[b0 + tid];
+        bias = a.bias_values[b0 + tid];
+    }
+    constexpr int AHEAD = 4;
+    int4 next[AHEAD];
+    if (counts && hvec) {
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int i = q0 / 4 + tid + 256 * k;
+            if (i < q1 / 4) next[k] = reinterpret_cast<const int4*>(a.history)[i];
+        }
+    }
     const int head = vec ? min(n, (int)(-base & 3)) : n, groups = (n - head) / 4;      // (without `vec` all are the first threads' besides)
 
     // the logits and their bits are on their way while the history is counted
@@ -95,27 +126,28 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     }
     if (counts) {
         for (int i = tid; i < RUN / 4; i += 256) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
-        for (int i = tid; i < RUN / 32; i += 256) touched[i] = 0;
         __syncthreads();
         auto count = [&](int token, bool output) {
             const int at = token - v0;
             if (at >= 0 && at < n) {
                 if (output) atomicAdd(&cnt[at], 1u);
                 else atomicOr(&cnt[at], ADJUST_SEEN);
-                atomicOr(&touched[at >> 5], 1u << (at & 31));
             }
         };
-        const int h0 = min(max(a.cu_history[r], 0), a.history_len), h1 = min(max(a.cu_history[r + 1], h0), a.history_len);
-        const int out0 = h0 + min(max(a.prompt_lens[r], 0), h1 - h0);
-        const int q0 = min(h1, (h0 + 3) & ~3), q1 = max(q0, h1 & ~3);      // (the part that int4 loads can take)
-        const bool hvec = ((uintptr_t)a.history & 15) == 0;
         if (hvec) {
-            for (int i = q0 / 4 + tid; i < q1 / 4; i += 256) {
-                const int4 h = reinterpret_cast<const int4*>(a.history)[i];
-                count(h.x, 4 * i >= out0);
-                count(h.y, 4 * i + 1 >= out0);
-                count(h.z, 4 * i + 2 >= out0);
-                count(h.w, 4 * i + 3 >= out0);
+            for (int i0 = q0 / 4; i0 < q1 / 4; i0 += 256 * AHEAD) {
+#pragma unroll
+                for (int k = 0; k < AHEAD; ++k) {
+                    const int i = i0 + tid + 256 * k, later = i + 256 * AHEAD;
+                    const int4 h = next[k];
+                    if (later < q1 / 4) next[k] = reinterpret_cast<const int4*>(a.history)[later];
+                    if (i < q1 / 4) {
+                        count(h.x, 4 * i >= out0);
+                        count(h.y, 4 * i + 1 >= out0);
+                        count(h.z, 4 * i + 2 >= out0);
+                        count(h.w, 4 * i + 3 >= out0);
+                    }
+                }
             }
             if (tid < 8) {
                 const int i = tid < 4 ? h0 + tid : q1 + tid - 4;
@@ -143,18 +175,19 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     for (int k = 0; k < PER; ++k) {
         const int j = tid + 256 * k, i = head + 4 * j;
         if (j >= groups) continue;
-        uint32_t some = 0;
-        if (counts) some = __funnelshift_r(touched[i >> 5], touched[min((i >> 5) + 1, RUN / 32 - 1)], i & 31) & 15u;
+        uint4 c = make_uint4(0, 0, 0, 0);
+        if (counts) c = head ? make_uint4(cnt[i], cnt[i + 1], cnt[i + 2], cnt[i + 3]) : *reinterpret_cast<const uint4*>(&cnt[i]);
+        const bool some = (c.x | c.y) | (c.z | c.w);
         if (in_place && allowed[k] == 15u && !some) continue;
         float4 z = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         if (allowed[k]) {
             z = v[k];
             if (in_place) z = *reinterpret_cast<const float4*>(x + i);
             if (some) {
-                z.x = adjusted(z.x, cnt[i]);
-                z.y = adjusted(z.y, cnt[i + 1]);
-                z.z = adjusted(z.z, cnt[i + 2]);
-                z.w = adjusted(z.w, cnt[i + 3]);
+                z.x = adjusted(z.x, c.x);
+                z.y = adjusted(z.y, c.y);
+                z.z = adjusted(z.z, c.z);
+                z.w = adjusted(z.w, c.w);
             }
             if (!(allowed[k] & 1)) z.x = -INFINITY;
             if (!(allowed[k] & 2)) z.y = -INFINITY;
@@ -171,26 +204,25 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     };
     for (int i = tid; i < head; i += 256) one(i);
     for (int i = head + 4 * groups + tid; i < n; i += 256) one(i);
-    if (a.cu_bias && has_request) {
+    if (b0 < b1) {
         // of equal tokens the last one listed counts: the largest place among them wins, by an integer maximum
-        const int b0 = min(max(a.cu_bias[r], 0), a.bias_len), b1 = min(max(a.cu_bias[r + 1], b0), a.bias_len);
-        if (b0 < b1) {
-            __syncthreads();
-            for (int i = b0 + tid; i < b1; i += 256) {
-                const int at = a.bias_ids[i] - v0;
-                if (at >= 0 && at < n) cnt[at] = 0;
+        auto each_bias = [&](auto f) {
+            int at = bias_id - v0;
+            if (b0 + tid < b1 && at >= 0 && at < n) f(at, tid, bias_id, bias);
+            for (int i = b0 + 256 + tid; i < b1; i += 256) {
+                const int z = a.bias_ids[i];
+                at = z - v0;
+                if (at >= 0 && at < n) f(at, i - b0, z, a.bias_values[i]);
             }
-            __syncthreads();
-            for (int i = b0 + tid; i < b1; i += 256) {
-                const int at = a.bias_ids[i] - v0;
-                if (at >= 0 && at < n) atomicMax(&cnt[at], (uint32_t)(i - b0 + 1));
-            }
-            __syncthreads();
-            for (int i = b0 + tid; i < b1; i += 256) {
-                const int z = a.bias_ids[i], at = z - v0;
-                if (at >= 0 && at < n && cnt[at] == (uint32_t)(i - b0 + 1) && (!mask || ((mask[z >> 5] >> (z & 31)) & 1))) y[at] += a.bias_values[i];
-            }
-        }
+        };
+        __syncthreads();
+        each_bias([&](int at, int, int, float) { cnt[at] = 0; });
+        __syncthreads();
+        each_bias([&](int at, int i, int, float) { atomicMax(&cnt[at], (uint32_t)(i + 1)); });
+        __syncthreads();
+        each_bias([&](int at, int i, int z, float value) {
+            if (cnt[at] == (uint32_t)(i + 1) && (!mask || ((mask[z >> 5] >> (z & 31)) & 1))) y[at] += value;
+        });
     }
 }
 
@@ -210,12 +242,14 @@ TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, 
     TFF_REQUIRE(cu_nodes || rows == requests, "adjust_logits: %d rows of %d requests", rows, requests);
     // Runs of 8,192 tokens, or of 2,048 where those would leave CUs without a block: every run goes through the request's whole history, so few and
     // long ones are better as soon as they fill the chip.
-    const int run = (int64_t)rows * ((V + 8191) / 8192) >= tff_device_cus() ? 8192 : 2048, runs = (V + run - 1) / run;
+    const int64_t eights = (int64_t)rows * ((V + 8191) / 8192);
+    const int run = eights >= 4 * tff_device_cus() ? 8192 : eights >= tff_device_cus() ? 4096 : 2048, runs = (V + run - 1) / run;
     TFF_REQUIRE((int64_t)rows * runs <= 0x7fffffff, "adjust_logits: %d rows of %d logits are more than a launch takes", rows, V);
     const AdjustArgs a{logits, out, rows, V, runs, history, cu_history, prompt_lens, history_len, requests, repetition, presence, frequency,
                        bias_ids, bias_values, cu_bias, bias_len, masks, masks ? num_masks : 0, (V + 31) / 32, mask_rows, draft_tokens, cu_nodes, ancestors, words};
     const int vec = (((uintptr_t)logits | (uintptr_t)out) & 15) == 0;      // (rows of both then begin alike)
     if (run == 8192) adjust_logits_kernel<8192><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a, vec);
+    else if (run == 4096) adjust_logits_kernel<4096><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a, vec);
     else adjust_logits_kernel<2048><<<rows * runs, 256, 0, (hipStream_t)stream>>>(a, vec);
     return tff_check_launch("adjust_logits");
 }
