@@ -153,7 +153,6 @@ __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
     return run;
 }
 
-// csrc/tree_attention_wide.hip: the plan's column tiles a wave (0: not its sizes), its launch
+// tree_attention_wide.hip: column tiles that a wave of it has at most for requests of so many columns (0: it is not for them), and its launch
 int tree_wide_tiles(int columns, int d);
-int tree_wide_blocks_per_cu(int d, int tiles);
-int tree_wide_launch(const TreeArgs& a, int d, int tiles, hipStream_t stream);
+int tree_wide_launch(const TreeArgs& a, int d, hipStream_t stream);

@@ -590,7 +590,6 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
         p.wide = 1;
         p.tiles = tree_wide_tiles(cols, d);
         p.columns = 64 * p.tiles;
-        per_cu = tree_wide_blocks_per_cu(d, p.tiles);
         p.least = 4;
     } else {
         p.tiles = cols <= 16 || d == 256 ? 1 : 2;      // (two tiles of a head of 256 are more than the registers hold)
@@ -657,17 +656,10 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
         TFF_TREE_MERGE(TT, SL, D, 16 * CT);                                          \
     } while (0)
         if (p.wide) {
-            if (int rc = tree_wide_launch(a, d, p.tiles, s)) return rc;
-#define TFF_TREE_WIDE(D)                                                      \
-    do {                                                                      \
-        if (p.tiles == 1) TFF_TREE_MERGE(bf16_t, 32, D, 64);                  \
-        if (p.tiles == 2) TFF_TREE_MERGE(bf16_t, 32, D, 128);                 \
-        TFF_TREE_MERGE(bf16_t, 32, D, 256);                                   \
-    } while (0)
-            if (d == 64) TFF_TREE_WIDE(64);
-            if (d == 128) TFF_TREE_WIDE(128);
-            TFF_TREE_WIDE(256);
-#undef TFF_TREE_WIDE
+            if (int rc = tree_wide_launch(a, d, s)) return rc;
+            if (d == 64) TFF_TREE_MERGE(bf16_t, 32, 64, 256);
+            if (d == 128) TFF_TREE_MERGE(bf16_t, 32, 128, 256);
+            TFF_TREE_MERGE(bf16_t, 32, 256, 128);
         }
 #define TFF_TREE_TILES(TT, SL)                                   \
     do {                                                         \

@@ -59,17 +59,14 @@ template <int N, typename F>
 __device__ __forceinline__ void each(F&& f) {
     each_of(f, std::make_integer_sequence<int, N>{});
 }
-// ring slots and blocks a CU: what the registers and LDS allow
+// slices of keys and values that LDS holds
 constexpr int ring_of(int d) { return d == 256 ? 4 : 8; }
-constexpr int blocks_of(int d, int tiles) { return d == 64 && tiles <= 2 ? 2 : 1; }
 
 template <int D, int CT, bool CAP>
-__global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const TreeArgs a) {
+__global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
     constexpr int COLS = 64 * CT, KS = D / 32, DT = D / 16, NR = ring_of(D);
     constexpr int KFR = 2 * KS, KC = KFR / 4, VC = DT / 4, CPI = KC + VC;      // fragments of a slice's keys, a wave's copies a step
     constexpr unsigned K_SLOT = KFR * 1024u, V_SLOT = DT * 1024u, V_BASE = NR * K_SLOT;
-    constexpr int NPV = (DT + 1) * CT, NQK = KFR * CT, NS = NPV + NQK;         // a step's MFMAs (the sums' among them)
-    constexpr int NP = 4 * CT, ITEMS = 3 * NP;                       // pairs of scores a lane, three instructions' worth each
     constexpr float LAG = 8.f;
     __shared__ __attribute__((aligned(1024))) char smem[V_BASE + NR * V_SLOT];
     __shared__ int32_t pages[TREE_PAGES];
@@ -124,10 +121,15 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
         static_assert(COLS <= 256, "a thread a column");
         const TreeRow row = tree_row(a.ancestors + (size_t)(t.n0 + (min(tid & (COLS - 1), ncols - 1) + group * COLS) / G) * a.words, a.words,
                                      t.end - t.start, t.start, a.window);
-        bf16x8 q[CT][KS];
+        // A wave's column tiles are every fourth: waves have as much to do whatever the columns, and a step is as long as the tiles there are.
+        auto run_of = [&](auto TILES) INLINE {
+        constexpr int NT = decltype(TILES)::value;
+        constexpr int NPV = (DT + 1) * NT, NQK = KFR * NT, NS = NPV + NQK;         // a step's MFMAs (the sums' among them)
+        constexpr int NP = 4 * NT, ITEMS = 3 * NP;                                 // pairs of scores a lane, three instructions' worth each
+        bf16x8 q[NT][KS];
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            const int c = min((wave * CT + ct) * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
+        for (int ct = 0; ct < NT; ++ct) {
+            const int c = min((ct * 4 + wave) * 16 + qc, ncols - 1) + group * COLS, node = c / G, head = g * G + (c - node * G);
             const bf16_t* qp = (const bf16_t*)a.q + (size_t)(t.n0 + node) * a.q_stride + (size_t)head * D + kg * 8;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) q[ct][ks] = *reinterpret_cast<const bf16x8*>(qp + ks * 32);
@@ -140,21 +142,21 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
             first_seen[tid] = row.lo;
         }
 
-        floatx4 o[CT][DT + 1], sc[2][CT][2];         // (the last of o: the sums, four times the same)
-        bf16x8 pf[2][CT], kf[KFR], vf[DT], ones;
-        float top_ref[CT], limit[CT], neg_ref[CT], factor[CT];  // a column's reference, what a score may be, minus the reference in the exponent's units, what the outputs still want
+        floatx4 o[NT][DT + 1], sc[2][NT][2];         // (the last of o: the sums, four times the same)
+        bf16x8 pf[2][NT], kf[KFR], vf[DT], ones;
+        float top_ref[NT], limit[NT], neg_ref[NT], factor[NT];  // a column's reference, what a score may be, minus the reference in the exponent's units, what the outputs still want
         bool rescale = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ones[i] = (bf16_t)1.f;
         hold(ones);                      // (in registers from here on: made anew right before an MFMA, which the compiler does not know for one, they came too late)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
+        for (int ct = 0; ct < NT; ++ct) {
             top_ref[ct] = limit[ct] = -INFINITY;
             neg_ref[ct] = 0.f;
             factor[ct] = 1.f;
         }
-        each<CT * (DT + 1)>([&](auto I) INLINE {
-            floatx4& x = o[decltype(I)::value % CT][decltype(I)::value / CT];
+        each<NT * (DT + 1)>([&](auto I) INLINE {
+            floatx4& x = o[decltype(I)::value % NT][decltype(I)::value / NT];
             x = floatx4{0.f, 0.f, 0.f, 0.f};
             pin(x);
         });
@@ -162,7 +164,7 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
 
         // which of the places key, key + 1, ... a column sees: a bit each (the next 8 of them hold)
         auto visible = [&](int ct, int key) INLINE {
-            const int c = (wave * CT + ct) * 16 + qc, j = key - t.start;
+            const int c = (ct * 4 + wave) * 16 + qc, j = key - t.start;
             const uint32_t* row = see + c * (TREE_WORDS + 1);
             if (j >= 0) {
                 const int w = min(j >> 5, TREE_WORDS - 1);
@@ -171,27 +173,27 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
             const int cached = min(-j, 31), below = min(max(first_seen[c] - key, 0), 31);
             return (((1u << cached) - 1) & (~0u << below)) | (-j < 32 ? row[0] << -j : 0u);
         };
-        auto settle = [&](floatx4 (&x)[CT][2]) INLINE {
+        auto settle = [&](floatx4 (&x)[NT][2]) INLINE {
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) asm volatile("" : "+v"(x[ct][0]), "+v"(x[ct][1]));
+            for (int ct = 0; ct < NT; ++ct) asm volatile("" : "+v"(x[ct][0]), "+v"(x[ct][1]));
         };
         // the first place of slice s; behind the run's last slice one that nobody sees
         auto place_of = [&](int s) INLINE { return s < s1 ? t.first + s * 32 : 0x40000000; };
         auto is_masked = [&](int k0) INLINE { return k0 + 32 > t.start || k0 < lo_most; };
-        auto mask = [&](floatx4 (&x)[CT][2], int k0) INLINE {
+        auto mask = [&](floatx4 (&x)[NT][2], int k0) INLINE {
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
+            for (int ct = 0; ct < NT; ++ct) {
                 const uint32_t sees = visible(ct, k0 + kg * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[ct][e >> 2][e & 3] = (sees >> e) & 1 ? x[ct][e >> 2][e & 3] : -INFINITY;
                 asm volatile("" : "+v"(x[ct][0]), "+v"(x[ct][1]));      // (here, in the branch)
             }
         };
-        auto cap = [&](floatx4 (&x)[CT][2]) INLINE {
+        auto cap = [&](floatx4 (&x)[NT][2]) INLINE {
             // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, as a score of its size is anyway
             const float in = -2.f * fabsf(a.scale) / a.softcap * log2e, outer = a.softcap * log2e;
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
+            for (int ct = 0; ct < NT; ++ct) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float s = x[ct][e >> 2][e & 3], z = __builtin_amdgcn_exp2f(-fabsf(s * in));
@@ -245,21 +247,21 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                     int page = bt[key >> a.page_shift];
                     if ((unsigned)page >= (unsigned)a.num_pages) page = 0;
                     const bf16_t* vp = vc + (size_t)page * (page_bytes / 2) + (key & (a.page_size - 1)) + (size_t)(4 * kg) * a.page_size;
-                    uint32_t sees[CT];
+                    uint32_t sees[NT];
 #pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) sees[ct] = visible(ct, key);
+                    for (int ct = 0; ct < NT; ++ct) sees[ct] = visible(ct, key);
                     each<DT>([&](auto F) INLINE {
                         constexpr int dt = decltype(F)::value;
                         each<4>([&](auto E) INLINE {
                             constexpr int e = decltype(E)::value;
                             const float x = to_f32(*vp);
                             vp += e < 3 ? a.page_size : 13 * a.page_size;
-                            each<CT>([&](auto C) INLINE {
+                            each<NT>([&](auto C) INLINE {
                                 constexpr int ct = decltype(C)::value;
                                 if ((sees[ct] & 1) && !(fabsf(x) < INFINITY)) o[ct][dt][e] += x;
                             });
                         });
-                        each<CT>([&](auto C) INLINE { pin(o[decltype(C)::value][dt]); });
+                        each<NT>([&](auto C) INLINE { pin(o[decltype(C)::value][dt]); });
                     });
                 }
             }
@@ -329,7 +331,7 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
             }
             if (c0 == s0) {
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct)
+                for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         uint4 x = __builtin_bit_cast(uint4, q[ct][ks]);
@@ -344,13 +346,13 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                 const char* src = smem + lane * 16;
                 each<KFR>([&](auto F) INLINE { kf[decltype(F)::value] = *reinterpret_cast<const bf16x8*>(src + decltype(F)::value * 1024); });
                 each<NQK>([&](auto I) INLINE {
-                    constexpr int f = decltype(I)::value / CT, ct = decltype(I)::value % CT, kt = f & 1, ks = f >> 1;
+                    constexpr int f = decltype(I)::value / NT, ct = decltype(I)::value % NT, kt = f & 1, ks = f >> 1;
                     if constexpr (ks == 0) score_first(sc[0][ct][kt], kf[kt * KS + ks], q[ct][ks]);
                     else score_next(sc[0][ct][kt], kf[kt * KS + ks], q[ct][ks]);
                 });
                 const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) pf[1][ct] = __builtin_bit_cast(bf16x8, zero);
+                for (int ct = 0; ct < NT; ++ct) pf[1][ct] = __builtin_bit_cast(bf16x8, zero);
                 each<DT>([&](auto F) INLINE { vf[decltype(F)::value] = __builtin_bit_cast(bf16x8, zero); });
                 asm volatile("s_nop 3");
             }
@@ -372,11 +374,11 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                 each<NS>([&](auto slot) INLINE {
                     constexpr int n_ = decltype(slot)::value;
                     if constexpr (n_ < NPV) {
-                        constexpr int ct = n_ % CT, dt = n_ / CT;
+                        constexpr int ct = n_ % NT, dt = n_ / NT;
                         if constexpr (dt < DT) mfma_acc(o[ct][dt], vf[dt], pf[h ^ 1][ct]);
                         else mfma_acc(o[ct][DT], ones, pf[h ^ 1][ct]);
                     } else {
-                        constexpr int f = (n_ - NPV) / CT, ct = (n_ - NPV) % CT, kt = f & 1, ks = f >> 1;
+                        constexpr int f = (n_ - NPV) / NT, ct = (n_ - NPV) % NT, kt = f & 1, ks = f >> 1;
                         if constexpr (ks == 0) score_first(sc[h ^ 1][ct][kt], kf[kt * KS + ks], q[ct][ks]);
                         else score_next(sc[h ^ 1][ct][kt], kf[kt * KS + ks], q[ct][ks]);
                     }
@@ -393,10 +395,10 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                     if constexpr (n_ == 4) {
                         if constexpr (CAP) cap(sc[h]);
                         if (is_masked(k0)) mask(sc[h], k0);
-                        float top[CT];
+                        float top[NT];
                         bool ahead = false;
 #pragma unroll
-                        for (int ct = 0; ct < CT; ++ct) {
+                        for (int ct = 0; ct < NT; ++ct) {
                             const floatx4 &x = sc[h][ct][0], &y = sc[h][ct][1];
                             top[ct] = largest3(largest3(x[0], x[1], x[2]), largest3(x[3], y[0], y[1]), largest3(y[2], y[3], y[3]));
                             ahead |= top[ct] > limit[ct];
@@ -404,7 +406,7 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                         if (__any(ahead)) {
                             rescale = true;
 #pragma unroll
-                            for (int ct = 0; ct < CT; ++ct) {
+                            for (int ct = 0; ct < NT; ++ct) {
                                 const float m = rows_max(top[ct]);
                                 const bool up = m > limit[ct];
                                 factor[ct] = up ? __builtin_amdgcn_exp2f((top_ref[ct] - m) * sl2) : 1.f;
@@ -447,12 +449,12 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                 });
                 // (worked out here: the compiler would move the softmax out of the MFMAs, behind the next step's branch)
 #pragma unroll
-                for (int ct = 0; ct < CT; ++ct) asm volatile("" : "+v"(pf[h][ct]));
+                for (int ct = 0; ct < NT; ++ct) asm volatile("" : "+v"(pf[h][ct]));
                 if (rescale) {
                     // the outputs hold the slices before s - 1 and s - 1 itself, all against the reference before
                     asm volatile("s_nop 15\n\ts_nop 15");
-                    each<CT*(DT + 1)>([&](auto I) INLINE {
-                        constexpr int ct = decltype(I)::value % CT, dt = decltype(I)::value / CT;
+                    each<NT*(DT + 1)>([&](auto I) INLINE {
+                        constexpr int ct = decltype(I)::value % NT, dt = decltype(I)::value / NT;
                         pin(o[ct][dt]);
                         o[ct][dt] *= factor[ct];
                         pin(o[ct][dt]);
@@ -477,21 +479,21 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
             if (is_masked(last)) clean(last);
             asm volatile("s_nop 3");
             each<NPV>([&](auto I) INLINE {
-                constexpr int ct = decltype(I)::value % CT, dt = decltype(I)::value / CT;
+                constexpr int ct = decltype(I)::value % NT, dt = decltype(I)::value / NT;
                 if constexpr (dt < DT) mfma_acc(o[ct][dt], vf[dt], pf[1][ct]);
                 else mfma_acc(o[ct][DT], ones, pf[1][ct]);
             });
         }
         __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(0));      // (the copies past the end must not outlive the block)
         asm volatile("s_nop 15\n\ts_nop 15");                // (the outputs' last MFMAs have written)
-        each<CT*(DT + 1)>([&](auto I) INLINE { pin(o[decltype(I)::value % CT][decltype(I)::value / CT]); });
+        each<NT*(DT + 1)>([&](auto I) INLINE { pin(o[decltype(I)::value % NT][decltype(I)::value / NT]); });
 
         const bool whole = s0 == 0 && s1 == t.slices;
         const size_t part = (((size_t)g * a.blocks + b) * 2 + (u == u0 ? 0 : 1)) * COLS;
         const int lane2 = w4_lane(), qc2 = lane2 & 15, kg2 = lane2 >> 4;
-        each<CT>([&](auto C) INLINE {
+        each<NT>([&](auto C) INLINE {
             constexpr int ct = decltype(C)::value;
-            const int c = (wave * CT + ct) * 16 + qc2;
+            const int c = (ct * 4 + wave) * 16 + qc2;
             if (c < ncols) {
                 float sum = o[ct][DT][0];
                 const float top = top_ref[ct] == -INFINITY ? -INFINITY : -neg_ref[ct];
@@ -518,19 +520,26 @@ __global__ __launch_bounds__(256, blocks_of(D, CT)) void tree_wide_kernel(const 
                 }
             }
         });
+        };
+        const int nt = (ncols + 63) / 64;
+        if constexpr (CT >= 4) {
+            if (nt == 4) run_of(std::integral_constant<int, 4>{});
+            else if (nt == 3) run_of(std::integral_constant<int, 3>{});
+        }
+        if constexpr (CT >= 2) {
+            if (nt == 2) run_of(std::integral_constant<int, 2>{});
+        }
+        if (nt == 1) run_of(std::integral_constant<int, 1>{});
         u += s1 - s0;
     }
 }
 
 }  // namespace
 
-int tree_wide_tiles(int columns, int d) {
-    if (columns <= 32) return 0;
-    return columns <= 64 ? 1 : columns <= 128 || d == 256 ? 2 : 4;
-}
-int tree_wide_blocks_per_cu(int d, int tiles) { return blocks_of(d, tiles); }
+// (up to 32 columns all waves have all of them, tree_attention.hip; a head of 256 leaves registers for half as many)
+int tree_wide_tiles(int columns, int d) { return columns <= 32 ? 0 : d == 256 ? 2 : 4; }
 
-int tree_wide_launch(const TreeArgs& a, int d, int tiles, hipStream_t stream) {
+int tree_wide_launch(const TreeArgs& a, int d, hipStream_t stream) {
     const int grid = tree_grid(a.nkv, a.blocks);
 #define TFF_TREE_W(D, CT)                                                                       \
     do {                                                                                        \
@@ -538,14 +547,9 @@ int tree_wide_launch(const TreeArgs& a, int d, int tiles, hipStream_t stream) {
         else tree_wide_kernel<D, CT, false><<<grid, 256, 0, stream>>>(a);                       \
         return tff_check_launch("tree_attention");                                              \
     } while (0)
-    if (d == 64 && tiles == 1) TFF_TREE_W(64, 1);
-    if (d == 64 && tiles == 2) TFF_TREE_W(64, 2);
-    if (d == 64 && tiles == 4) TFF_TREE_W(64, 4);
-    if (d == 128 && tiles == 1) TFF_TREE_W(128, 1);
-    if (d == 128 && tiles == 2) TFF_TREE_W(128, 2);
-    if (d == 128 && tiles == 4) TFF_TREE_W(128, 4);
-    if (d == 256 && tiles == 1) TFF_TREE_W(256, 1);
-    if (d == 256 && tiles == 2) TFF_TREE_W(256, 2);
+    if (d == 64) TFF_TREE_W(64, 4);
+    if (d == 128) TFF_TREE_W(128, 4);
+    if (d == 256) TFF_TREE_W(256, 2);
 #undef TFF_TREE_W
-    return tff_fail("tree_attention: no kernel for head size %d and %d column tiles a wave", d, tiles);
+    return tff_fail("tree_attention: no kernel for head size %d", d);
 }
