@@ -509,12 +509,16 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
     }
 }
 
-// The partial results of a group of columns, in the order of the keys: a wave a (node, q head).
-template <typename T, int SLICE, int D, int COLS>
+// The partial results of a group of columns, in the order of the keys: a wave has H q heads of a node, and 8 / H partial results of each on their way
+// together.  A wave waits for memory four times one after the other, whatever it merges, so H is 4 where single heads would be more waves than the
+// GPU holds twice (870 nodes of 40 heads: 23.6 us with single heads, 18 so; 42 nodes of 16: 4.4, and 8).
+#define MERGE_HEADS 4
+template <typename T, int SLICE, int D, int COLS, int H>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
-    constexpr int N = D / 64;
-    const int row = blockIdx.x, lane = threadIdx.x & 63, head = blockIdx.y * 4 + (threadIdx.x >> 6), G = a.nq / a.nkv;
-    if (head >= a.nq) return;
+    constexpr int N = D / 64, J = 8 / H;
+    const int row = blockIdx.x, lane = threadIdx.x & 63, G = a.nq / a.nkv;
+    const int head0 = (blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * H;
+    if (head0 >= a.nq) return;
     // the row's request, the units before it and all of them, in one pass over the tables
     int r = 0, total = 0, before = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
@@ -534,46 +538,80 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
     if (node < 0 || node >= t.nodes) return;
     const int share = tree_share(total, a.blocks, a.least);
     const float log2e = 1.4426950408889634f;
-    const int g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
-    const int u0 = before + group * t.slices, u1 = u0 + t.slices;
-    const int b0 = u0 / share, b1 = (u1 - 1) / share;
-    if (b0 == b1) return;                        // (one block had all of it, and wrote the result)
-    auto part_of = [&](int b) { return (((size_t)g * a.blocks + b) * 2 + (b == b0 && u0 != b * share ? 1 : 0)) * COLS + c; };
-    float top = -INFINITY, sum = 0.f, acc[N];
+    // per head: its first partial result (elements of part_o in units of D), how many, from which on they follow each other
+    long long first[H], rest[H];
+    int n[H], most = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
-    for (int b = b0 + lane; b <= b1; b += 64) top = fmaxf(top, a.part_ml[part_of(b) * 2]);
-    top = wave_max(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    for (int c0 = b0; c0 <= b1; c0 += 64) {
-        const int n = min(64, b1 - c0 + 1);
-        const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[part_of(c0 + min(lane, n - 1))];
-        const float f = lane < n ? __builtin_amdgcn_exp2f(ml.x - ref) : 0.f;
-        sum += wave_sum(lane < n ? ml.y * f : 0.f);
-        for (int i0 = 0; i0 < n; i0 += 4) {      // (four at a time: their loads together)
-            float o[4][N], w[4];
+    for (int k = 0; k < H; ++k) {
+        const int head = min(head0 + k, a.nq - 1), g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
+        const int u0 = before + group * t.slices, b0 = u0 / share, b1 = (u0 + t.slices - 1) / share;
+        const long long base = (long long)g * a.blocks * 2 * COLS + c;
+        first[k] = base + ((long long)b0 * 2 + (u0 != b0 * share ? 1 : 0)) * COLS;
+        rest[k] = base + (long long)b0 * 2 * COLS;
+        n[k] = head0 + k < a.nq && b0 != b1 ? b1 - b0 + 1 : 0;         // (one block had all of it, and wrote the result)
+        most = max(most, n[k]);
+    }
+    if (most == 0) return;
+    auto part_of = [&](int k, int i) { return i == 0 ? first[k] : rest[k] + (long long)i * 2 * COLS; };
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+    float top[H], sum[H], acc[H][N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* p = a.part_o + part_of(c0 + min(i0 + i, n - 1)) * D + lane;
+    for (int k = 0; k < H; ++k) {
+        top[k] = -INFINITY;
+        sum[k] = 0.f;
 #pragma unroll
-                for (int k = 0; k < N; ++k) o[i][k] = p[k * 64];
-                w[i] = i0 + i < n ? __shfl(f, min(i0 + i, 63), 64) : 0.f;
-            }
+        for (int i = 0; i < N; ++i) acc[k][i] = 0.f;
+    }
+    for (int c0 = 0; c0 < most; c0 += 64) {
+        // (64 partial results at a time, against the largest reference so far)
+        float2 v[H];
+        float f[H];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < H; ++k) v[k] = c0 + lane < n[k] ? ml[part_of(k, c0 + lane)] : make_float2(-INFINITY, 0.f);
 #pragma unroll
-                for (int k = 0; k < N; ++k) acc[k] += i0 + i < n ? o[i][k] * w[i] : 0.f;
+        for (int k = 0; k < H; ++k) {
+            const float now = fmaxf(top[k], wave_max(v[k].x)), ref = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f(top[k] - ref);
+            f[k] = __builtin_amdgcn_exp2f(v[k].x - ref);
+            sum[k] = sum[k] * old + wave_sum(v[k].y * f[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[k][i] *= old;
+            top[k] = now;
+        }
+        const int m = min(64, most - c0);
+        for (int i0 = 0; i0 < m; i0 += J) {
+            float o[J][H][N];
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int k = 0; k < H; ++k) {
+                    // (past a head's last: the last once more, with a weight of zero)
+                    const float* p = a.part_o + part_of(k, min(c0 + i0 + j, max(n[k] - 1, 0))) * D + lane;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) o[j][k][i] = n[k] > 0 ? p[i * 64] : 0.f;
+                }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int k = 0; k < H; ++k) {
+                    const float w = __shfl(f[k], min(i0 + j, 63), 64);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc[k][i] += c0 + i0 + j < n[k] ? o[j][k][i] * w : 0.f;
+                }
         }
     }
-    if (a.sinks) {
-        const float sink = a.sinks[head] * log2e;
-        if (top == -INFINITY) sum = 1.f;
-        else sum += __builtin_amdgcn_exp2f(sink - top);
-    }
-    const float inv = sum > 0.f ? 1.0f / sum : sum != sum ? sum : 0.f;
-    T* op = (T*)a.out + ((size_t)row * a.nq + head) * D;
 #pragma unroll
-    for (int i = 0; i < N; ++i) op[i * 64 + lane] = from_f32<T>(acc[i] * inv);
+    for (int k = 0; k < H; ++k) {
+        if (n[k] == 0) continue;
+        if (a.sinks) {
+            const float sink = a.sinks[head0 + k] * log2e;
+            if (top[k] == -INFINITY) sum[k] = 1.f;
+            else sum[k] += __builtin_amdgcn_exp2f(sink - top[k]);
+        }
+        const float inv = sum[k] > 0.f ? 1.0f / sum[k] : sum[k] != sum[k] ? sum[k] : 0.f;
+        T* op = (T*)a.out + ((size_t)row * a.nq + head0 + k) * D;
+#pragma unroll
+        for (int i = 0; i < N; ++i) op[i * 64 + lane] = from_f32<T>(acc[k][i] * inv);
+    }
 }
 
 // The launch's shape: column tiles of a block (narrow: all of them in every wave; wide: of each wave), blocks a kv head, units a block
@@ -641,12 +679,14 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
         const TreeArgs a{q, k_cache, v_cache, out, block_tables, cu_nodes, start_pos, ancestors, sinks, part_o,
                          part_o + (size_t)nkv * p.blocks * 2 * p.columns * d, q_stride, bt_stride, words, R, rows, nq, nkv, page_size, shift,
                          num_pages, window, p.blocks, p.least, scale, softcap};
-        const dim3 merge(rows, (nq + 3) / 4);
+        const int heads = (int64_t)rows * nq > 2 * 32 * (int64_t)tff_device_cus() ? MERGE_HEADS : 1;      // (a CU holds 32 waves)
+        const dim3 merge(rows, (nq + 4 * heads - 1) / (4 * heads));
         // (a block a kv head has every run whole)
 #define TFF_TREE_MERGE(TT, SL, D, COLS)                                       \
     do {                                                                      \
         if (p.blocks == 1) return 0;                                          \
-        tree_merge_kernel<TT, SL, D, COLS><<<merge, 256, 0, s>>>(a);          \
+        if (heads == 1) tree_merge_kernel<TT, SL, D, COLS, 1><<<merge, 256, 0, s>>>(a); \
+        else tree_merge_kernel<TT, SL, D, COLS, MERGE_HEADS><<<merge, 256, 0, s>>>(a);  \
         return tff_check_launch("tree_merge");                                \
     } while (0)
 #define TFF_TREE_MM(TT, SL, D, CT, OCC)                                              \

@@ -369,7 +369,10 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
                 const char* vsrc = smem + V_BASE + v_rd + lane * 16;
                 const int k0 = slice_place(s), prev = s > 0 ? slice_place(s - 1) : 0;
                 if (s > 0 && is_masked(prev)) clean(prev);
-                float tmp0 = 0.f, tmp1 = 0.f;
+                float tmp0 = 0.f, tmp1 = 0.f, top[NT];
+                bool ahead = false;
+                constexpr bool SPREAD = NS >= 16;                     // the maxima go between the MFMAs, too, where there are enough of these
+                constexpr int CHECK = SPREAD ? 5 + 4 * NT : 4;
                 unsigned long long ka = 0, va = 0;
                 each<NS>([&](auto slot) INLINE {
                     constexpr int n_ = decltype(slot)::value;
@@ -395,14 +398,21 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
                     if constexpr (n_ == 4) {
                         if constexpr (CAP) cap(sc[h]);
                         if (is_masked(k0)) mask(sc[h], k0);
-                        float top[NT];
-                        bool ahead = false;
-#pragma unroll
-                        for (int ct = 0; ct < NT; ++ct) {
+                    }
+                    each<4 * NT>([&](auto I) INLINE {
+                        constexpr int ct = decltype(I)::value / 4, j = decltype(I)::value % 4;
+                        if constexpr (n_ == (SPREAD ? 5 + decltype(I)::value : 4)) {
                             const floatx4 &x = sc[h][ct][0], &y = sc[h][ct][1];
-                            top[ct] = largest3(largest3(x[0], x[1], x[2]), largest3(x[3], y[0], y[1]), largest3(y[2], y[3], y[3]));
-                            ahead |= top[ct] > limit[ct];
+                            if constexpr (j == 0) top[ct] = largest3(x[0], x[1], x[2]);
+                            else if constexpr (j == 1) top[ct] = largest3(top[ct], x[3], y[0]);
+                            else if constexpr (j == 2) top[ct] = largest3(top[ct], y[1], y[2]);
+                            else {
+                                top[ct] = largest3(top[ct], y[3], y[3]);
+                                ahead |= top[ct] > limit[ct];
+                            }
                         }
+                    });
+                    if constexpr (n_ == CHECK) {
                         if (__any(ahead)) {
                             rescale = true;
 #pragma unroll
@@ -417,8 +427,8 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
                             }
                         }
                     }
-                    if constexpr (n_ > 4) {
-                        constexpr int i0 = (n_ - 5) * ITEMS / (NS - 5), i1 = (n_ - 4) * ITEMS / (NS - 5);
+                    if constexpr (n_ > CHECK) {
+                        constexpr int i0 = (n_ - CHECK - 1) * ITEMS / (NS - CHECK - 1), i1 = (n_ - CHECK) * ITEMS / (NS - CHECK - 1);
                         each<i1 - i0>([&](auto I) INLINE {
                             constexpr int i = i0 + decltype(I)::value, p = i / 3, ct = p / 4, e = (p % 4) * 2;
                             if constexpr (i % 3 == 0) {
