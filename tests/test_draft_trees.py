@@ -24,6 +24,7 @@ ATTENTION = dict(q=P, q_stride=256, out=P, k=P, v=P, bt=P, bt_stride=4, cu=P, st
     (dict(nkv=0), "multiple"), (dict(d=0), "head size"), (dict(d=513), "head size"), (dict(page=0), "geometry"), (dict(pages=0), "geometry"),
     (dict(bt_stride=0), "geometry"), (dict(window=-1), "geometry"), (dict(softcap=-1.0), "geometry"), (dict(words=0), "words"),
     (dict(words=9), "words"), (dict(q_stride=255), "stride"), (dict(dtype=2), "dtype"), (dict(rows=-1), "sizes"), (dict(R=-1), "sizes"),
+    (dict(bt_stride=1 << 20, page=4096), "tables of"), (dict(), "overlaps"), (dict(out=P + 3 * 512 - 2), "overlaps"), (dict(out=P - 3 * 512 + 2), "overlaps"),
 ])
 def test_tree_attention_refuses(change, what):
     _refused("tff_tree_attention", {**ATTENTION, **change}.values(), what)

@@ -60,18 +60,18 @@ def attention_tol(dtype, d, places, out, out_abs, most):
 
 
 def check_attention(nq, nkv, d, page, dtype, starts, trees, window=0, softcap=0.0, sinks=False, sees=None, words=None, rest=math.nan, seed=0, qscale=2.0,
-                    poison=None, scale=None, extra=0):
-    """trees: parents by request; sees: the nodes' bits where they are no paths.  ``extra`` rows behind the last node."""
+                    poison=None, scale=None, extra=0, before=0):
+    """trees: parents by request; sees: the nodes' bits where they are no paths.  ``extra`` rows behind the last node, ``before`` ones before the first."""
     sees = sees or [plain.paths(t) for t in trees]
     cache = Cache([s + len(t) for s, t in zip(starts, sees)], nkv, d, page, dtype, rest, seed)
     if poison is not None:
         poison(cache)
-    cu = [0]
+    cu = [before]
     for t in sees:
         cu.append(cu[-1] + len(t))
     words = words or max(1, -(-max(len(t) for t in sees) // 32))
     q = (qscale * torch.randn(cu[-1] + extra, nq * d)).to(dtype)
-    bits = plain.packed([row for t in sees for row in t] + [[0]] * extra, words)
+    bits = plain.packed([[0]] * before + [row for t in sees for row in t] + [[0]] * extra, words)
     sink = torch.randn(nq) if sinks else None
     kc, vc, table = cache.gpu()
     out = torch.full((cu[-1] + extra, nq * d), 7.0, dtype=dtype, device=DEV)
@@ -80,7 +80,7 @@ def check_attention(nq, nkv, d, page, dtype, starts, trees, window=0, softcap=0.
     got = ops.tree_attention(*args, **kw, out=out)
     assert got.data_ptr() == out.data_ptr()
     got = got.cpu()
-    assert bool((got[cu[-1]:] == 7.0).all())
+    assert bool((got[cu[-1]:] == 7.0).all()) and bool((got[:before] == 7.0).all())
     worst = 0.0
     for r, s in enumerate(starts):
         n = len(sees[r])
@@ -98,7 +98,7 @@ def check_attention(nq, nkv, d, page, dtype, starts, trees, window=0, softcap=0.
         if err.numel():
             worst = max(worst, float(err.max()))
     assert worst <= 1.0, worst
-    if not extra:
+    if not extra and not before:
         assert torch.equal(ops.tree_attention(*args, **kw).cpu().view(torch.int16 if dtype == BF16 else torch.int32),
                            got.view(torch.int16 if dtype == BF16 else torch.int32))
 
@@ -185,6 +185,57 @@ def test_attention_of_many_requests_of_uneven_lengths():
     starts = [rng.choice((0, 3, 60, 200, 700, 1500)) for _ in range(70)]
     check_attention(2, 1, 64, 16, BF16, starts, some_trees(rng, [rng.randint(1, 9) for _ in starts]))
     check_attention(2, 1, 64, 16, F32, starts[:20], some_trees(rng, [rng.randint(1, 9) for _ in starts[:20]]))
+
+
+@pytest.mark.parametrize("nq, dtype, n", [(8, BF16, 2), (8, BF16, 40), (4, F32, 3)])
+def test_attention_of_a_long_cache(nq, dtype, n):
+    """More partial results of a group of columns than a wave has lanes, and pages of many tokens."""
+    check_attention(nq, 1, 128, 256, dtype, [20000], some_trees(random.Random(n), [n]))
+    check_attention(nq, 1, 64, 16, dtype, [9001], some_trees(random.Random(n), [n]), window=8600, sinks=True)
+
+
+@pytest.mark.parametrize("d, page", [(64, 64), (128, 128), (256, 8)])
+def test_attention_of_many_wide_requests(d, page):
+    """More requests than a wave has lanes, of many columns: blocks that begin and end in the middle of a request, and requests without nodes."""
+    rng = random.Random(d)
+    starts = [rng.choice((0, 3, 60, 200, 700)) for _ in range(70)]
+    check_attention(16, 1, d, page, BF16, starts, some_trees(rng, [rng.choice((0, 1, 5, 9)) for _ in starts], 4), window=0 if d == 64 else 90)
+
+
+def test_attention_of_more_pages_than_a_block_holds_numbers_of():
+    """As many kv heads as the GPU has CUs, small pages: a block goes through a whole request of more pages than LDS has room for."""
+    nkv, d, page, start, n = 256, 64, 8, 9000, 20
+    k, v = torch.randn(40, nkv, page, d).to(BF16), torch.randn(40, nkv, d, page).to(BF16)
+    table = torch.randint(0, 40, (1, -(-(start + n) // page)), dtype=torch.int32)
+    q = torch.randn(n, 2 * nkv * d).to(BF16)
+    see = plain.paths(plain.random_tree(random.Random(1), n, 6))
+    got = ops.tree_attention(q.to(DEV), 2 * nkv, nkv, d, k.to(DEV), v.to(DEV), table.to(DEV), ints([0, n]), ints([start]), plain.packed(see, 1).to(DEV))
+    got = got.cpu().double().view(n, 2 * nkv, d)
+    for g in (0, 101, 255):
+        keys, values = k[table[0].long(), g].reshape(-1, 1, d), v[table[0].long(), g].transpose(1, 2).reshape(-1, 1, d)
+        heads = slice(2 * g, 2 * g + 2)
+        o, o_abs, most = plain.attention(q.view(n, 2 * nkv, d)[:, heads], keys, values, start, see, 2, 1)
+        assert bool(((got[:, heads] - o).abs() <= attention_tol(BF16, d, start + n, o, o_abs, most)).all()), g
+
+
+@pytest.mark.parametrize("nq, d", [(4, 80), (4, 64), (40, 128)])
+def test_attention_leaves_rows_that_no_request_has(nq, d):
+    """Rows before the first node and behind the last, and nodes for which the ancestors have no bits."""
+    check_attention(nq, 2, d, 16, BF16, [5, 90], some_trees(random.Random(1), [6, 3]), extra=4, before=3)
+    q, k, v = (torch.randn(s, device=DEV).to(BF16) for s in ((40, nq * d), (4, 2, 16, d), (4, 2, d, 16)))
+    out = torch.full((40, nq * d), 7.0, dtype=BF16, device=DEV)
+    ops.tree_attention(q, nq, 2, d, k, v, ints([[3, 1, 0, 2]]), ints([0, 40]), ints([9]), torch.ones(40, 1, dtype=torch.int32, device=DEV), out=out)
+    assert bool((out[32:] == 7.0).all()) and not bool((out[:32] == 7.0).all(1).any())
+
+
+def test_attention_window_of_any_size():
+    q, k, v = (torch.randn(s, device=DEV).to(BF16) for s in ((3, 256), (4, 2, 16, 64), (4, 2, 64, 16)))
+    args = (q, 4, 2, 64, k, v, ints([[3, 1, 0, 2]]), ints([0, 3]), ints([40]), ints([[1], [3], [5]]))
+    every = ops.tree_attention(*args)
+    for window in (42, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(ops.tree_attention(*args, window=window), every)
+    with pytest.raises(KernelError):
+        ops.tree_attention(*args, window=-(1 << 32))
 
 
 def test_attention_of_large_scores():
@@ -289,6 +340,14 @@ def test_adjust_rows_of_trees(V, n):
     for in_place in (False, True):
         check_adjust(4, V, [20, 0, 3, 0], [10, 0, 0, 0], PENS[2:], None, masks, [rng.randrange(-1, 2) for _ in range(rows)], trees, in_place)
         check_adjust(4, V, [20, 0, 3, 0], [10, 0, 0, 0], PENS[2:], [[(3, 1.0)], [], [(V - 1, -2.0)], []], trees=trees, in_place=in_place)
+
+
+def test_adjust_leaves_rows_that_no_request_has():
+    x, f = torch.randn(7, 3000, device=DEV), torch.full((2,), 2.0, device=DEV)
+    tokens, cu, bits = ints([5] * 7), ints([2, 3, 5]), ints([[1]] * 7)
+    masks = (torch.zeros(1, 94, dtype=torch.int32, device=DEV), ints([0] * 7))
+    got = ops.adjust_logits(x, ints([7, 9]), ints([0, 1, 2]), ints([1, 0]), f, f, f, masks=masks, drafts=(tokens, cu, bits))
+    assert torch.equal(got[:2], x[:2]) and torch.equal(got[5:], x[5:]) and bool((got[2:5] == -math.inf).all())
 
 
 def test_adjust_values_that_are_not_finite():
@@ -401,7 +460,7 @@ def test_refusals():
     for bad in (dict(q=q[:, :100]), dict(q=q.float()), dict(q=q.t()), dict(k=v), dict(v=v.float()), dict(table=table.long()), dict(table=ints([[0, 1]] * 2)),
                 dict(cu=ints([0, 3, 3])), dict(bits=ints([1, 3, 5])), dict(bits=bits[:2]), dict(bits=torch.zeros(3, 9, dtype=torch.int32, device=DEV)),
                 dict(bits=bits.long()), dict(start=start.cpu()), dict(sinks=torch.zeros(3, device=DEV)), dict(window=-1), dict(softcap=-2.0),
-                dict(out=torch.zeros(3, 64, dtype=BF16, device=DEV)), dict(q=torch.zeros(3, 96, dtype=BF16, device=DEV), nq=3)):
+                dict(out=torch.zeros(3, 64, dtype=BF16, device=DEV)), dict(out=q), dict(q=torch.zeros(3, 96, dtype=BF16, device=DEV), nq=3)):
         with pytest.raises(KernelError):
             attention(**bad)
     x, f = torch.zeros(2, 40, device=DEV), torch.ones(2, device=DEV)
@@ -421,7 +480,8 @@ def test_refusals():
         with pytest.raises(KernelError):
             ops.tree_accept(*args)
     path, n = ints([[0, 2]]), ints([2])
-    for args in (([(k, k)], table, start, path, n), ([(k, v), (k, v)], table, start, path, n), ([(k, v), (k.float(), v.float())], table, start, path, n),
+    both = torch.zeros(6, 2, 16, 32, dtype=BF16, device=DEV)
+    for args in (([(both[:4], v), (both[2:], v.clone())], table, start, path, n), ([(k, k)], table, start, path, n), ([(k, v), (k, v)], table, start, path, n), ([(k, v), (k.float(), v.float())], table, start, path, n),
                  ([(k, v)], table, start, path[0], n), ([(k, v)], table, start, path, ints([1, 2])), ([(k, v)], ints([[0], [1]]), start, path, n),
                  ([(k, v)], table, start, torch.zeros(1, 257, dtype=torch.int32, device=DEV), n), ([(k.cpu(), v.cpu())], table, start, path, n)):
         with pytest.raises(KernelError):
@@ -605,3 +665,35 @@ def test_captured_and_on_another_stream():
         for x, y in zip(held, together(ek, ev)):
             assert torch.equal(x, y), i
         assert torch.equal(gk, ek) and torch.equal(gv, ev)
+
+
+def test_two_streams_at_once():
+    """Calls of one shape on two streams, in flight together, give what they give one after the other."""
+    rng = random.Random(8)
+    trees, starts, nq, nkv, d, page = some_trees(rng, [30, 9, 12]), [3000, 50, 900], 16, 2, 128, 16
+    cu, bits = ints([0, 30, 39, 51]), plain.packed([p for t in trees for p in plain.paths(t)], 1).to(DEV)
+    sides = []
+    for seed in range(2):
+        k, v, table = Cache([s + len(t) for s, t in zip(starts, trees)], nkv, d, page, BF16, 0.0, seed).gpu()
+        q, x = torch.randn(51, nq * d, device=DEV).to(BF16), torch.randn(51, 20000, device=DEV)
+        hist = ints([rng.randrange(20000) for _ in range(4000)])
+        sides.append((q, k, v, table, x, hist))
+    pen, three, cuh = torch.full((3,), 1.3, device=DEV), ints(starts), ints([0, 3000, 3050, 3950])
+
+    def step(q, k, v, table, x, hist):
+        o = ops.tree_attention(q, nq, nkv, d, k, v, table, cu, three, bits)
+        y = ops.adjust_logits(x, hist, cuh, three, pen, pen, pen, drafts=(hist[:51].contiguous(), cu, bits))
+        return o, y, *ops.tree_accept(ops.argmax(y), hist[:51].contiguous(), cu, bits, 5)
+    alone = [step(*s) for s in sides]
+    streams = [torch.cuda.Stream() for _ in sides]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*sides[i]))
+    torch.cuda.synchronize()
+    for i, want in enumerate(alone):
+        for g in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(g, want))

@@ -13,6 +13,7 @@
 // option touches is neither.  The bound is memory: 4 bytes a logit in and out.
 #include "common.h"
 #include "tffinfer_kernels.h"
+#include "tree_attention.h"
 
 #define ADJUST_SEEN 0x80000000u      // in the prompt; the bits below count the output
 
@@ -34,16 +35,6 @@ struct AdjustArgs {
     int words;
 };
 
-// The request that row t belongs to, the same in every lane: as many of cu[1 .. n] as are not behind t (n: to none).
-__device__ __forceinline__ int row_request(const int32_t* __restrict__ cu, int n, int t) {
-    int upto = 0;
-    for (int r0 = 0; r0 < n; r0 += 64) {
-        const int r = r0 + (int)(threadIdx.x & 63);
-        upto += __popcll(__ballot(r < n && cu[min(r, n - 1) + 1] <= t));
-    }
-    return upto;
-}
-
 // Four bits of a mask from token v on (the words behind the last are not read).
 __device__ __forceinline__ uint32_t mask_bits4(const int32_t* __restrict__ mask, int words, int v) {
     const int w = v >> 5;
@@ -63,9 +54,9 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     const bool in_place = a.logits == a.out;
     const int mask_row = a.mask_rows ? a.mask_rows[t] : -1;
     int r = t;
-    if (a.cu_nodes) r = row_request(a.cu_nodes, a.requests, t);
+    if (a.cu_nodes) r = tree_row_request(a.cu_nodes, a.requests, t);
     r = __builtin_amdgcn_readfirstlane(r);
-    const bool has_request = r < a.requests;      // (a row behind the last node is left as it is)
+    const bool has_request = r < a.requests;      // (a row that no request has is left as it is)
     const int32_t* __restrict__ mask = has_request && mask_row >= 0 && mask_row < a.num_masks ? a.masks + (size_t)mask_row * a.mask_words : nullptr;
     // (all that the rest hangs on, asked for at once)
     float rep = 1.f, pres = 0.f, freq = 0.f;
@@ -128,8 +119,8 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
         for (int i = tid; i < RUN / 4; i += 256) reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
         auto count = [&](int token, bool output) {
-            const int at = token - v0;
-            if (at >= 0 && at < n) {
+            const unsigned at = (unsigned)token - (unsigned)v0;
+            if (at < (unsigned)n) {
                 if (output) atomicAdd(&cnt[at], 1u);
                 else atomicOr(&cnt[at], ADJUST_SEEN);
             }

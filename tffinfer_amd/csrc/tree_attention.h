@@ -6,12 +6,12 @@
 
 // The request that row t belongs to, the same in every lane: as many of cu[1 .. n] as are not behind t (n: to none).
 __device__ __forceinline__ int tree_row_request(const int32_t* __restrict__ cu, int n, int t) {
-    int upto = 0;
+    int upto = t < cu[0] ? n : 0;
     for (int r0 = 0; r0 < n; r0 += 64) {
         const int r = r0 + (int)(threadIdx.x & 63);
         upto += __popcll(__ballot(r < n && cu[min(r, n - 1) + 1] <= t));
     }
-    return upto;
+    return min(upto, n);
 }
 
 // What a node sees of its tree (bits of nodes that the request has not are dropped, and under a window the first ones), and the first cached place.

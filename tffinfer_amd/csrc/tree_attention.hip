@@ -23,7 +23,7 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
     __shared__ long long voff[64];
     const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, g = h / (nq / nkv);
     const int r = tree_row_request(cu_nodes, R, t);
-    if (r >= R) return;                          // (a row behind the last node is left as it is)
+    if (r >= R || t - max(cu_nodes[r], 0) >= 32 * words) return;      // (a row that no request has is left as it is)
     const int nodes = min(cu_nodes[r + 1], rows) - max(cu_nodes[r], 0);
     const long long room = (long long)bt_stride * page_size;
     const int start = (int)min((long long)max(start_pos[r], 0), room), end = (int)min((long long)start + min(nodes, 32 * words), room);
@@ -666,8 +666,11 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
     TFF_REQUIRE(dtype == TFF_F32 || dtype == TFF_BF16, "tree_attention: unknown dtype %d", dtype);
     if (rows == 0 || R == 0) return 0;
     TFF_REQUIRE(q && out && k_cache && v_cache && block_tables && cu_nodes && start_pos && ancestors, "tree_attention: null pointer");
+    TFF_REQUIRE((int64_t)bt_stride * page_size < 0x40000000, "tree_attention: tables of %d pages of %d tokens", bt_stride, page_size);
     hipStream_t s = (hipStream_t)stream;
     const int esz = dtype == TFF_F32 ? 4 : 2;
+    const uintptr_t q0 = (uintptr_t)q, q1 = q0 + (size_t)rows * q_stride * esz, o0 = (uintptr_t)out, o1 = o0 + (size_t)rows * nq * d * esz;
+    TFF_REQUIRE(o1 <= q0 || q1 <= o0, "tree_attention: the output overlaps the queries");      // (a block reads queries after others have written)
     const size_t need = tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
     if (need > 0 && workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0 && ((uintptr_t)q & 15) == 0 &&
         ((size_t)q_stride * esz) % 16 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0) {

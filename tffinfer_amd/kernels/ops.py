@@ -2713,7 +2713,7 @@ def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Te
     """Attention of trees of drafted tokens: rows ``cu_nodes[r]:cu_nodes[r + 1]`` of ``q`` [rows, >= nq * d] are request r's nodes, whose
     keys and values lie in its pages from place ``start_pos[r]`` on (as :func:`qk_norm_rope_kv` puts them there, at positions by their
     depth).  A node sees the places before and the nodes whose bit its row of ``ancestors`` (int32 [rows, words], 32 nodes a word,
-    lowest bit first, its own among them) has; under a ``window`` the last so many of these.  ``sinks`` (float32 [nq]) and ``softcap``:
+    lowest bit first, its own among them) has; under a ``window`` the last so many of these (0: all).  ``sinks`` (float32 [nq]) and ``softcap``:
     see :func:`paged_attention`.  Returns [rows, nq * d] in q's type, which is the cache's; a node that sees nothing gets zeros, rows that
     no request has are left as they are.  Up to 256 nodes a request, head sizes up to 512; a token's bits may depend on what else is in the
     step, as they do where decoding splits keys.  The table of pages has to reach to a request's last node."""
@@ -2743,12 +2743,15 @@ def tree_attention(q: torch.Tensor, nq: int, nkv: int, d: int, k_cache: torch.Te
             raise _lib.KernelError(f"tree_attention out: shape {tuple(out.shape)} is not {(rows, nq * d)}")
     if scale is None:
         scale = 1.0 / math.sqrt(d)
+    window = min(int(window), 0x7fffffff)
+    if window < 0:
+        raise _lib.KernelError(f"tree_attention: window {window}")
     L, code, tables_width = _lib.load(), dtype_code(dtype), block_tables.shape[1]
     room = _tree_workspace(rows, R, nq, nkv, d, page_size, tables_width, code, dev)
     ws = torch.empty(room, dtype=torch.uint8, device=q.device) if room else None
     _lib.check(L.tff_tree_attention(
         qp, width, out.data_ptr(), kp, vp, table, tables_width, cu, start, bits, ancestors.shape[1], R, rows, nq, nkv, d, page_size, pages,
-        int(window), float(scale), sink, float(softcap or 0.0), _ptr(ws), room, code, _stream()))
+        window, float(scale), sink, float(softcap or 0.0), _ptr(ws), room, code, _stream()))
     return out
 
 
@@ -2808,8 +2811,9 @@ def cache_keep(caches: list, block_tables: torch.Tensor, start_pos: torch.Tensor
                 raise _lib.KernelError(f"cache_keep: keys {tuple(k.shape)} beside {tuple(first.shape)}")
             _check_cache(k, v, nkv, d, what)
     at = list(map(_address, both))
-    if len(set(at)) != 2 * n:
-        raise _lib.KernelError("cache_keep: a cache is listed twice")
+    by_place, room = sorted(at), first.numel() * first.element_size()
+    if any(map(operator.gt, (x + room for x in by_place), by_place[1:])):
+        raise _lib.KernelError("cache_keep: a cache is listed twice, or overlaps another")
     ptrs = (ctypes.c_void_p * (2 * n))(*at)
     base = ctypes.addressof(ptrs)
     _lib.check(_lib.load().tff_cache_keep(base, base + 8 * n, n, table, block_tables.shape[1], start, places, kept, R, path.shape[1], nkv, d,
