@@ -56,10 +56,19 @@ struct TreeArgs {
     float scale, softcap;
 };
 
+// What work is dealt by: the weight of a slice of a group of so many columns, in ninths of a microsecond (a wide kernel's step by its tiles of 64
+// columns; a narrow one's columns are all the same to it), and of what a group takes beside its slices: a pipeline that fills, a partial
+// result or two.  (24 requests of 200 to 8,000 places and 1 to 48 nodes of 5 heads: 122 us with all slices and nothing else alike, 112.5 with 44, 110 with
+// 70; 8 requests of 2,048, whose groups are alike: 38.1, 37.1, 36.9, and 42 with 100.)
+template <int COLS>
+__host__ __device__ constexpr int tree_weight(int columns) { return COLS >= 128 ? 3 + 2 * ((columns + 63) / 64) : 1; }
+template <int COLS>
+__host__ __device__ constexpr int tree_begin() { return COLS >= 128 ? 70 : 0; }
+
 // One request's share of the work.
 struct TreeRequest {
     int n0, nodes, start, end, first;    // its first row, nodes, cached places, places, and the first place that a slice begins with
-    int slices, groups;
+    int slices, groups, last;            // (the weight of the last group's slices)
 };
 template <int SLICE, int COLS>
 __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
@@ -70,11 +79,30 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
     t.start = (int)min((long long)max(a.start_pos[r], 0), room);
     t.end = (int)min((long long)t.start + t.nodes, room);
     t.first = a.window > 0 ? max(0, t.start - a.window) / 32 * 32 : 0;
-    t.groups = (t.nodes * (a.nq / a.nkv) + COLS - 1) / COLS;
+    const int columns = t.nodes * (a.nq / a.nkv);
+    t.groups = (columns + COLS - 1) / COLS;
+    t.last = tree_weight<COLS>(columns - max(t.groups - 1, 0) * COLS);
     // (a request with nodes has a slice even where its table has no room for them: its rows are written)
     t.slices = t.nodes > 0 ? max(1, (t.end - t.first + SLICE - 1) / SLICE) : 0;
     return t;
 }
+template <int COLS>
+__device__ __forceinline__ int tree_cost(const TreeRequest& t) {
+    return t.slices > 0 ? t.groups * tree_begin<COLS>() + t.slices * ((t.groups - 1) * tree_weight<COLS>(COLS) + t.last) : 0;
+}
+// A group of a request: where it begins, the weight of its slices, and which slice is the first that begins at x or behind.
+template <int COLS>
+struct TreeGroup {
+    int at, weight;
+    __device__ __forceinline__ TreeGroup(const TreeRequest& t, int before, int group) {
+        at = before + group * (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
+        weight = group == t.groups - 1 ? t.last : tree_weight<COLS>(COLS);
+    }
+    __device__ __forceinline__ int begin(int s) const { return s == 0 ? at : at + tree_begin<COLS>() + s * weight; }
+    __device__ __forceinline__ int slice(int x) const {
+        return x <= at ? 0 : max(1, (x - at - tree_begin<COLS>() + weight - 1) / weight);
+    }
+};
 __device__ __forceinline__ int tree_wave_scan(int v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -85,23 +113,20 @@ __device__ __forceinline__ int tree_wave_scan(int v) {
     return v;
 }
 
-// Units of all requests, and of those before request `upto`; the same in every lane.
+// The weight of all requests, and of those before request `upto`; the same in every lane.
 template <int SLICE, int COLS>
 __device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& total, int& before) {
     total = before = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         const int r = r0 + (int)(threadIdx.x & 63);
         int u = 0;
-        if (r < a.R) {
-            const TreeRequest t = tree_request<SLICE, COLS>(a, r);
-            u = t.slices * t.groups;
-        }
+        if (r < a.R) u = tree_cost<COLS>(tree_request<SLICE, COLS>(a, r));
         const int incl = tree_wave_scan(u);
         if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
         total += __builtin_amdgcn_readlane(incl, 63);
     }
 }
-// How many units a block takes: an equal share, and no less than `least` (a block has its loads to wait for before the first).
+// What a block takes: an equal share, and no less than `least` (a block has its loads to wait for before the first slice).
 __device__ __forceinline__ int tree_share(int total, int blocks, int least) { return max((total + blocks - 1) / blocks, least); }
 
 // Which run and kv head a block of the launch has: eight runs by eight, within them the kv heads, within a kv head the eight runs.  Blocks go
@@ -113,9 +138,9 @@ __device__ __forceinline__ void tree_place(int nkv, int& b, int& g) {
 }
 static inline int tree_grid(int nkv, int blocks) { return nkv * ((blocks + 7) / 8 * 8); }
 
-// Block b's run of units u0 .. u1 - 1, the request that it begins in and the units before that request; the same in every lane.
+// Block b's share x0 .. x1 - 1 (it has the slices that begin there), the request that x0 is in and the weight before it; the same in every lane.
 struct TreeRun {
-    int u0, u1, r, before;
+    int x0, x1, r, before;
     TreeRequest t;
 };
 template <int SLICE, int COLS>
@@ -127,18 +152,18 @@ __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
     run.r = run.before = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
-        const int u = r0 + lane < a.R ? t.slices * t.groups : 0, incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
+        const int u = r0 + lane < a.R ? tree_cost<COLS>(t) : 0, incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
         if (r0 == 0) {
             if (a.R <= 64) total = all;
             const int share = tree_share(total, a.blocks, a.least);
-            run.u0 = min(total, b * share);
-            run.u1 = min(total, run.u0 + share);
+            run.x0 = min(total, b * share);
+            run.x1 = min(total, run.x0 + share);
         }
-        if (run.before + all <= run.u0) {
+        if (run.before + all <= run.x0) {
             run.before += all;
             continue;
         }
-        const int at = __ffsll((long long)__ballot(run.before + incl > run.u0)) - 1;
+        const int at = __ffsll((long long)__ballot(run.before + incl > run.x0)) - 1;
         run.r = r0 + at;
         run.before += __builtin_amdgcn_readlane(incl - u, at);
         run.t.n0 = __builtin_amdgcn_readlane(t.n0, at);
@@ -148,6 +173,7 @@ __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
         run.t.first = __builtin_amdgcn_readlane(t.first, at);
         run.t.slices = __builtin_amdgcn_readlane(t.slices, at);
         run.t.groups = __builtin_amdgcn_readlane(t.groups, at);
+        run.t.last = __builtin_amdgcn_readlane(t.last, at);
         break;
     }
     return run;

@@ -236,19 +236,22 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
 
     // the block's run of units, and the request that it begins in
     const TreeRun run = tree_run<SLICE, COLS>(a, b);
-    const int u0 = run.u0, u1 = run.u1;
-    if (u0 >= u1) return;
+    const int x1 = run.x1;
+    if (run.x0 >= x1) return;
     int r = run.r, before = run.before;
     TreeRequest t = run.t;
 
-    for (int u = u0; u < u1;) {
-        if (u >= before + t.slices * t.groups) {
-            before += t.slices * t.groups;
+    for (int x = run.x0; x < x1;) {
+        if (x >= before + tree_cost<COLS>(t)) {
+            before += tree_cost<COLS>(t);
             t = tree_request<SLICE, COLS>(a, ++r);
             continue;
         }
-        const int group = (u - before) / t.slices, s0 = u - before - group * t.slices;
-        const int s1 = min(t.slices, s0 + (u1 - u));
+        const int group = (x - before) / (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
+        const TreeGroup<COLS> span(t, before, group);
+        const int s0 = span.slice(x), s1 = min(t.slices, span.slice(x1));
+        x = span.begin(t.slices);
+        if (s0 >= s1) continue;          // (x is in the last slice, the block's before)
         const int ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
 
@@ -469,7 +472,7 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
         }
         __syncthreads();
         const bool whole = s0 == 0 && s1 == t.slices;
-        const size_t part = (((size_t)g * a.blocks + b) * 2 + (u == u0 ? 0 : 1)) * COLS;
+        const size_t part = (((size_t)g * a.blocks + b) * 2 + (s0 == 0 ? 1 : 0)) * COLS;
         for (int i = tid2; i < ncols * (D / 4); i += 256) {
             const int c = i / (D / 4), e = (i - c * (D / 4)) * 4;
             float top = merge_m[c];
@@ -505,7 +508,6 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
                 }
             }
         }
-        u += s1 - s0;
     }
 }
 
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         const TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
         const bool in = r0 + lane < a.R;
-        const int u = in ? t.slices * t.groups : 0, incl = tree_wave_scan(u);
+        const int u = in ? tree_cost<COLS>(t) : 0, incl = tree_wave_scan(u);
         const int behind = __popcll(__ballot(in && a.cu_nodes[min(r0 + lane, a.R - 1) + 1] <= row));
         if (r == r0) {
             if (behind > 0) before += __builtin_amdgcn_readlane(incl, behind - 1);
@@ -544,9 +546,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
 #pragma unroll
     for (int k = 0; k < H; ++k) {
         const int head = min(head0 + k, a.nq - 1), g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
-        const int u0 = before + group * t.slices, b0 = u0 / share, b1 = (u0 + t.slices - 1) / share;
+        const TreeGroup<COLS> from(t, before, group);
+        const int b0 = from.at / share, b1 = from.begin(t.slices - 1) / share;
         const long long base = (long long)g * a.blocks * 2 * COLS + c;
-        first[k] = base + ((long long)b0 * 2 + (u0 != b0 * share ? 1 : 0)) * COLS;
+        first[k] = base + ((long long)b0 * 2 + 1) * COLS;
         rest[k] = base + (long long)b0 * 2 * COLS;
         n[k] = head0 + k < a.nq && b0 != b1 ? b1 - b0 + 1 : 0;         // (one block had all of it, and wrote the result)
         most = max(most, n[k]);
@@ -617,10 +620,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
 // The launch's shape: column tiles of a block (narrow: all of them in every wave; wide: of each wave), blocks a kv head, units a block
 // takes at least; 0 tiles: the general kernel.
 struct TreePlan {
-    int wide, tiles, blocks, least, columns;
+    int wide, tiles, blocks, least, columns, weight, begin;
 };
 static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {
-    TreePlan p{0, 0, 0, 0, 0};
+    TreePlan p{0, 0, 0, 0, 0, 0, 0};
     if (!(d == 64 || d == 128 || d == 256) || page_size < 8 || page_size > 65536 || (page_size & (page_size - 1)) || nkv <= 0 || nq % nkv || R <= 0 || rows <= 0) return p;
     const int cols = (int)(((long long)rows * (nq / nkv) + R - 1) / R);      // a request's columns, on average
     int per_cu = 1;
@@ -628,8 +631,11 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
         p.wide = 1;
         p.tiles = tree_wide_tiles(cols, d);
         p.columns = 64 * p.tiles;
-        p.least = 4;
+        p.weight = d == 256 ? tree_weight<128>(128) : tree_weight<256>(256);
+        p.begin = tree_begin<256>();
+        p.least = 4 * p.weight + p.begin;
     } else {
+        p.weight = 1;
         p.tiles = cols <= 16 || d == 256 ? 1 : 2;      // (two tiles of a head of 256 are more than the registers hold)
         p.columns = 16 * p.tiles;
         if (d < 256) per_cu = 2;
@@ -638,8 +644,8 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
     }
     const int slice = dtype == TFF_F32 ? 16 : 32;
     const long long all = (long long)rows * (nq / nkv), most = (all > R ? all - R : 0) / p.columns + R;      // groups of columns, at most
-    const long long units = most * (((long long)bt_stride * page_size + slice - 1) / slice);
-    if (units > 0x3fffffff) return TreePlan{0, 0, 0, 0, 0};                  // (they are counted in 32 bits)
+    const long long units = most * (((long long)bt_stride * page_size + slice - 1) / slice * p.weight + p.begin);
+    if (units > 0x3fffffff) return TreePlan{0, 0, 0, 0, 0, 0, 0};                  // (they are counted in 32 bits)
     long long blocks = (long long)tff_device_cus() * per_cu / nkv;
     if (blocks < 1) blocks = 1;
     p.blocks = (int)(blocks < (units + p.least - 1) / p.least ? blocks : (units + p.least - 1) / p.least);

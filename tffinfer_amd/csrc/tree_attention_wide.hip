@@ -94,19 +94,23 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
     const unsigned v_step = (unsigned)a.page_size * 32u;                       // bytes from a value tile to the next
 
     const TreeRun run = tree_run<32, COLS>(a, b);
-    const int u0 = run.u0, u1 = run.u1;
-    if (u0 >= u1) return;
+    const int x1 = run.x1;
+    if (run.x0 >= x1) return;
     int r = run.r, before = run.before;
     TreeRequest t = run.t;
 
-    for (int u = u0; u < u1;) {
-        if (u >= before + t.slices * t.groups) {
-            before += t.slices * t.groups;
+    for (int x = run.x0; x < x1;) {
+        if (x >= before + tree_cost<COLS>(t)) {
+            before += tree_cost<COLS>(t);
             t = tree_request<32, COLS>(a, ++r);
             continue;
         }
-        const int group = (u - before) / t.slices, s0 = u - before - group * t.slices;
-        const int s1 = min(t.slices, s0 + (u1 - u)), ncols = min(COLS, t.nodes * G - group * COLS);
+        const int group = (x - before) / (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
+        const TreeGroup<COLS> span(t, before, group);
+        const int s0 = span.slice(x), s1 = min(t.slices, span.slice(x1));
+        x = span.begin(t.slices);
+        if (s0 >= s1) continue;          // (x is in the last slice, the block's before)
+        const int ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
 
         // The first chunk's page numbers, the columns' bits and the queries are asked for together.  (A chunk: slices whose page numbers fit,
@@ -499,7 +503,7 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
         each<NT*(DT + 1)>([&](auto I) INLINE { pin(o[decltype(I)::value % NT][decltype(I)::value / NT]); });
 
         const bool whole = s0 == 0 && s1 == t.slices;
-        const size_t part = (((size_t)g * a.blocks + b) * 2 + (u == u0 ? 0 : 1)) * COLS;
+        const size_t part = (((size_t)g * a.blocks + b) * 2 + (s0 == 0 ? 1 : 0)) * COLS;
         const int lane2 = w4_lane(), qc2 = lane2 & 15, kg2 = lane2 >> 4;
         each<NT>([&](auto C) INLINE {
             constexpr int ct = decltype(C)::value;
@@ -540,7 +544,6 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
             if (nt == 2) run_of(std::integral_constant<int, 2>{});
         }
         if (nt == 1) run_of(std::integral_constant<int, 1>{});
-        u += s1 - s0;
     }
 }
 
