@@ -8,7 +8,7 @@
 // From node 0 (the token the request already had) on: to the first child whose token is what the model chose after the node, until no
 // child is or `max_path` nodes are kept.  A node's parent is the last node that it sees before itself.  A wave a request: a lane
 // has the nodes lane, lane + 64, ..., and a level is a comparison and a ballot.  Bound by latency: two loads after each other, then
-// registers.
+// registers (2.2 us for one request of 8 nodes, 3.7 for 64 of up to 64).
 __global__ __launch_bounds__(64) void tree_accept_kernel(const int32_t* __restrict__ choices, const int32_t* __restrict__ tokens,
                                                          const int32_t* __restrict__ cu_nodes, const int32_t* __restrict__ ancestors,
                                                          int words, int T, int max_path, int32_t* __restrict__ path,
@@ -70,8 +70,9 @@ TFF_API int tff_tree_accept(const int32_t* choices, const int32_t* tokens, const
 // For request r and i < counts[r]: the key and value at place start_pos[r] + path[r, i] of its pages to place start_pos[r] + i, in all
 // caches of the call.  Whoever has an element of a head (eight of them, of a key) has it of all moves, and loads them all before it stores
 // any, so a place may be both a source and a target, whatever the path: up to KEEP_FEW moves in a thread's registers, more through LDS.
-// Values lie transposed ([element][place]): their moves are elements, 2 bytes of a sector each.  Bound by latency: the path, the pages, the data.
-// us for 32 requests with paths of up to 8 and 8 layers of 8 heads of 128, all moves through LDS, a block a head / this: 14 / 4.7.
+// Values lie transposed ([element][place]): their moves are elements, 2 bytes of a line of memory each.  Bound by latency (the path, the pages, the
+// data: 2.1 us for one request and 28 layers), and for many requests by the values' lines: 32 requests with paths of up to 8 and 8 layers of 8 heads
+// of 128 move 4 MB of keys and values and touch some 40; 14 us with all moves through LDS and a block a head, 10.4 so.
 #define KEEP_CACHES 64               // caches a launch takes: their pointers are its arguments
 #define KEEP_PATH 256                // kept places of a request, at most
 #define KEEP_FEW 8

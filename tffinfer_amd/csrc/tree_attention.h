@@ -56,13 +56,13 @@ struct TreeArgs {
     float scale, softcap;
 };
 
-// What work is dealt by: the weight of a slice of a group of so many columns, in ninths of a microsecond (a wide kernel's step by its tiles of 64
-// columns; a narrow one's columns are all the same to it), and of what a group takes beside its slices: a pipeline that fills, a partial
-// result or two.  (24 requests of 200 to 8,000 places and 1 to 48 nodes of 5 heads: 122 us with all slices and nothing else alike, 112.5 with 44, 110 with
+// What work is dealt by: the weight of a slice of a group of so many columns (wide: a step by its tiles of 64 columns, in ninths of a microsecond;
+// narrow: one, whatever the columns), and of what a run takes beside its slices: a pipeline that fills, a partial result.
+// (24 requests of 256 to 8,192 places and 24 to 48 nodes of 5 heads: 122 us with all slices and nothing else alike, 112.5 with a begin of 44, 110 with
 // 70; 8 requests of 2,048, whose groups are alike: 38.1, 37.1, 36.9, and 42 with 100.)
 template <int COLS>
 __host__ __device__ constexpr int tree_weight(int columns) { return COLS >= 128 ? 3 + 2 * ((columns + 63) / 64) : 1; }
-template <int COLS>
+template <int SLICE, int COLS>
 __host__ __device__ constexpr int tree_begin() { return COLS >= 128 ? 70 : 0; }
 
 // One request's share of the work.
@@ -86,21 +86,39 @@ __device__ __forceinline__ TreeRequest tree_request(const TreeArgs& a, int r) {
     t.slices = t.nodes > 0 ? max(1, (t.end - t.first + SLICE - 1) / SLICE) : 0;
     return t;
 }
-template <int COLS>
+template <int SLICE, int COLS>
 __device__ __forceinline__ int tree_cost(const TreeRequest& t) {
-    return t.slices > 0 ? t.groups * tree_begin<COLS>() + t.slices * ((t.groups - 1) * tree_weight<COLS>(COLS) + t.last) : 0;
+    return t.slices > 0 ? t.groups * tree_begin<SLICE, COLS>() + t.slices * ((t.groups - 1) * tree_weight<COLS>(COLS) + t.last) : 0;
 }
-// A group of a request: where it begins, the weight of its slices, and which slice is the first that begins at x or behind.
-template <int COLS>
+// A group of a request: its weight's begin, the weight of a slice, and the first slice of the block whose share begins at x.  A share that would
+// begin near the group's begin begins there, and one near its end behind it: what a block takes on for that is less than beginning once more and a
+// partial result (float32's slices are too slow for that).  us before / so: 8 requests of 300 places and 20 columns 27.7 / 15.9, 3 of 90 and 80
+// columns 29.0 / 17.7, 8 of 2,048 and 104 columns 37.1 / 33.6, 24 ragged ones 111 / 109.
+template <int SLICE, int COLS>
 struct TreeGroup {
-    int at, weight;
+    static constexpr int BEGIN = tree_begin<SLICE, COLS>(), NEAR = COLS >= 128 ? 44 : SLICE == 16 ? 1 : 8;
+    int at, weight, slices;
     __device__ __forceinline__ TreeGroup(const TreeRequest& t, int before, int group) {
-        at = before + group * (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
+        at = before + group * (BEGIN + t.slices * tree_weight<COLS>(COLS));
         weight = group == t.groups - 1 ? t.last : tree_weight<COLS>(COLS);
+        slices = t.slices;
     }
-    __device__ __forceinline__ int begin(int s) const { return s == 0 ? at : at + tree_begin<COLS>() + s * weight; }
+    __device__ __forceinline__ int end() const { return at + BEGIN + slices * weight; }
     __device__ __forceinline__ int slice(int x) const {
-        return x <= at ? 0 : max(1, (x - at - tree_begin<COLS>() + weight - 1) / weight);
+        if (x < at + NEAR) return 0;
+        if (x > end() - NEAR) return slices;
+        return max(1, (x - at - BEGIN + weight - 1) / weight);
+    }
+    // the blocks of its first slice and of its last
+    __device__ __forceinline__ int first_block(int share) const {
+        int b = at / share;
+        while ((b + 1) * share < min(end(), at + NEAR)) ++b;
+        return b;
+    }
+    __device__ __forceinline__ int last_block(int share) const {
+        int b = (end() - 1) / share;
+        while (b * share >= at + NEAR && b * share > end() - NEAR) --b;
+        return b;
     }
 };
 __device__ __forceinline__ int tree_wave_scan(int v) {
@@ -120,7 +138,7 @@ __device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& tot
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         const int r = r0 + (int)(threadIdx.x & 63);
         int u = 0;
-        if (r < a.R) u = tree_cost<COLS>(tree_request<SLICE, COLS>(a, r));
+        if (r < a.R) u = tree_cost<SLICE, COLS>(tree_request<SLICE, COLS>(a, r));
         const int incl = tree_wave_scan(u);
         if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
         total += __builtin_amdgcn_readlane(incl, 63);
@@ -152,7 +170,7 @@ __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
     run.r = run.before = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
-        const int u = r0 + lane < a.R ? tree_cost<COLS>(t) : 0, incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
+        const int u = r0 + lane < a.R ? tree_cost<SLICE, COLS>(t) : 0, incl = tree_wave_scan(u), all = __builtin_amdgcn_readlane(incl, 63);
         if (r0 == 0) {
             if (a.R <= 64) total = all;
             const int share = tree_share(total, a.blocks, a.least);

@@ -96,8 +96,8 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
 
 // ---- on the matrix cores: bfloat16 and float32, head sizes 64, 128 and 256, pages of a power of two of tokens, at least 8 ----
 // The columns of a request and kv head are its (node, q head of the group) pairs, node * G + head, in groups of 16 CT.  The work
-// is cut into units of one slice of keys (32 in bfloat16, 16 in float32) and one group of columns; every block finds out by itself, from the
-// requests' tables, which run of units is its own (total / blocks of them, consecutive: the slices of a group of columns, then the next
+// is cut into slices of keys (32 in bfloat16, 16 in float32) of one group of columns; every block finds out by itself, from the
+// requests' tables, which run of them is its own (an equal share of their weights, consecutive: the slices of a group of columns, then the next
 // group's, then the next request's), so that blocks end together whatever the requests' lengths, nothing is planned on the host and a
 // captured launch serves any lengths.  The four waves of a block take every fourth slice, with all the block's columns in
 // registers: a key or value goes from memory into the registers of one wave and into no other, no LDS and no barrier in the loop.  S^T = K Q^T
@@ -105,6 +105,8 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
 // scores' registers are the second product's operand as they lie.  The maximum that the exponentials are taken against follows the true one
 // when that is more than 2^8 ahead: the outputs are rescaled some times a run, not at every slice.  At a run's end the four waves meet in LDS; a
 // group of columns whose slices went to several blocks leaves a partial result with each, merged by a second kernel.
+// What bounds it: a few slices are latency (tables, pages, then the keys; 9.2 us for one request of 500 places and 26 columns, 1.3 MB), many the
+// memory (4 requests of 32,000 places and 32 columns: 109 us, 4.8 TB/s).  float32 runs at its own MFMAs' rate, 2 us a slice and wave.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 tree_bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float tree_f32x4;
 typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t tree_u32x4;
@@ -242,16 +244,16 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
     TreeRequest t = run.t;
 
     for (int x = run.x0; x < x1;) {
-        if (x >= before + tree_cost<COLS>(t)) {
-            before += tree_cost<COLS>(t);
+        if (x >= before + tree_cost<SLICE, COLS>(t)) {
+            before += tree_cost<SLICE, COLS>(t);
             t = tree_request<SLICE, COLS>(a, ++r);
             continue;
         }
-        const int group = (x - before) / (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
-        const TreeGroup<COLS> span(t, before, group);
-        const int s0 = span.slice(x), s1 = min(t.slices, span.slice(x1));
-        x = span.begin(t.slices);
-        if (s0 >= s1) continue;          // (x is in the last slice, the block's before)
+        const int group = (x - before) / (tree_begin<SLICE, COLS>() + t.slices * tree_weight<COLS>(COLS));
+        const TreeGroup<SLICE, COLS> span(t, before, group);
+        const int s0 = span.slice(x), s1 = x1 < span.end() ? span.slice(x1) : t.slices;
+        x = span.end();
+        if (s0 >= s1) continue;          // (another block has it)
         const int ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
 
@@ -526,7 +528,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         const TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
         const bool in = r0 + lane < a.R;
-        const int u = in ? tree_cost<COLS>(t) : 0, incl = tree_wave_scan(u);
+        const int u = in ? tree_cost<SLICE, COLS>(t) : 0, incl = tree_wave_scan(u);
         const int behind = __popcll(__ballot(in && a.cu_nodes[min(r0 + lane, a.R - 1) + 1] <= row));
         if (r == r0) {
             if (behind > 0) before += __builtin_amdgcn_readlane(incl, behind - 1);
@@ -542,16 +544,20 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
     const float log2e = 1.4426950408889634f;
     // per head: its first partial result (elements of part_o in units of D), how many, from which on they follow each other
     long long first[H], rest[H];
-    int n[H], most = 0;
+    int n[H], most = 0, which = -1, b0 = 0, b1 = 0;
 #pragma unroll
     for (int k = 0; k < H; ++k) {
         const int head = min(head0 + k, a.nq - 1), g = head / G, col = node * G + head - g * G, group = col / COLS, c = col - group * COLS;
-        const TreeGroup<COLS> from(t, before, group);
-        const int b0 = from.at / share, b1 = from.begin(t.slices - 1) / share;
+        if (group != which) {
+            const TreeGroup<SLICE, COLS> from(t, before, group);
+            b0 = from.first_block(share);
+            b1 = from.last_block(share);
+            which = group;
+        }
         const long long base = (long long)g * a.blocks * 2 * COLS + c;
         first[k] = base + ((long long)b0 * 2 + 1) * COLS;
         rest[k] = base + (long long)b0 * 2 * COLS;
-        n[k] = head0 + k < a.nq && b0 != b1 ? b1 - b0 + 1 : 0;         // (one block had all of it, and wrote the result)
+        n[k] = head0 + k < a.nq && b0 < b1 ? b1 - b0 + 1 : 0;         // (one block had all of it, and wrote the result)
         most = max(most, n[k]);
     }
     if (most == 0) return;
@@ -632,15 +638,16 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
         p.tiles = tree_wide_tiles(cols, d);
         p.columns = 64 * p.tiles;
         p.weight = d == 256 ? tree_weight<128>(128) : tree_weight<256>(256);
-        p.begin = tree_begin<256>();
+        p.begin = tree_begin<32, 256>();
         p.least = 4 * p.weight + p.begin;
     } else {
         p.weight = 1;
         p.tiles = cols <= 16 || d == 256 ? 1 : 2;      // (two tiles of a head of 256 are more than the registers hold)
         p.columns = 16 * p.tiles;
         if (d < 256) per_cu = 2;
-        // slices a wave: four where they are quick (a run that one block has whole needs no merge), one where float32's are not (2 us each)
-        p.least = dtype == TFF_F32 ? 4 : 16;
+        // slices a wave, at least: two where they are quick, one where float32's are not (2 us each).  us with 16 slices a block / 8, one request of 1,500
+        // places and 20 columns 19.0 / 15.6, 8 of 1,000 18.4 / 16.0
+        p.least = dtype == TFF_F32 ? 4 : 8;
     }
     const int slice = dtype == TFF_F32 ? 16 : 32;
     const long long all = (long long)rows * (nq / nkv), most = (all > R ? all - R : 0) / p.columns + R;      // groups of columns, at most
@@ -648,8 +655,8 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
     if (units > 0x3fffffff) return TreePlan{0, 0, 0, 0, 0, 0, 0};                  // (they are counted in 32 bits)
     long long blocks = (long long)tff_device_cus() * per_cu / nkv;
     if (blocks < 1) blocks = 1;
-    p.blocks = (int)(blocks < (units + p.least - 1) / p.least ? blocks : (units + p.least - 1) / p.least);
-    if (p.blocks < 1) p.blocks = 1;
+    if (blocks > (units + p.least - 1) / p.least) blocks = (units + p.least - 1) / p.least;
+    p.blocks = !p.wide && dtype == TFF_BF16 && units <= 16 ? 1 : (int)blocks;      // (what one block has whole needs no merge)
     return p;
 }
 TFF_API size_t tff_tree_attention_workspace_bytes(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {

@@ -1,5 +1,5 @@
-// bfloat16 attention of drafted trees for requests of many columns (node, q head of the group): the four waves of a block take 16 CT
-// columns each and share the keys and values, which travel into a ring of slices in LDS while earlier slices are worked on.  What
+// bfloat16 attention of drafted trees for requests of many columns (node, q head of the group): the four waves of a block take every fourth
+// tile of 16 columns, up to CT each, and share the keys and values, which travel into a ring of slices in LDS while earlier slices are worked on.  What
 // the columns are, how the work is dealt to blocks and what a partial result is: tree_attention.hip, whose kernel has every column in every
 // wave and so wants few of them.
 //
@@ -9,7 +9,8 @@
 // reduce a maximum nor rescale.  The sum of a column's weights is one more row of the second product (values of one): it is the sum of the
 // weights as they are rounded, so that a dominant weight's rounding cancels.
 // What bounds it: with 256 columns and a head of 128 the issue of a wave's 68 MFMAs, 32 exponentials and some 130 other instructions a
-// slice; with fewer columns the keys and values from memory.
+// slice; with fewer columns the keys and values from memory.  4 requests of 32,700 places (543 MB): 64 columns 113 us (4.8 TB/s, what a
+// copy reads and writes), 128 126, 192 141, 256 166 (717 TFLOP/s; the copies alone take 118, the arithmetic alone 135).
 #include <type_traits>
 #include <utility>
 
@@ -100,16 +101,16 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
     TreeRequest t = run.t;
 
     for (int x = run.x0; x < x1;) {
-        if (x >= before + tree_cost<COLS>(t)) {
-            before += tree_cost<COLS>(t);
+        if (x >= before + tree_cost<32, COLS>(t)) {
+            before += tree_cost<32, COLS>(t);
             t = tree_request<32, COLS>(a, ++r);
             continue;
         }
-        const int group = (x - before) / (tree_begin<COLS>() + t.slices * tree_weight<COLS>(COLS));
-        const TreeGroup<COLS> span(t, before, group);
-        const int s0 = span.slice(x), s1 = min(t.slices, span.slice(x1));
-        x = span.begin(t.slices);
-        if (s0 >= s1) continue;          // (x is in the last slice, the block's before)
+        const int group = (x - before) / (tree_begin<32, COLS>() + t.slices * tree_weight<COLS>(COLS));
+        const TreeGroup<32, COLS> span(t, before, group);
+        const int s0 = span.slice(x), s1 = x1 < span.end() ? span.slice(x1) : t.slices;
+        x = span.end();
+        if (s0 >= s1) continue;          // (another block has it)
         const int ncols = min(COLS, t.nodes * G - group * COLS);
         const int32_t* __restrict__ bt = a.block_tables + (size_t)r * a.bt_stride;
 
@@ -549,7 +550,8 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
 
 }  // namespace
 
-// (up to 32 columns all waves have all of them, tree_attention.hip; a head of 256 leaves registers for half as many)
+// Up to 32 columns all waves have all of them (tree_attention.hip): us here / there, one request of 200 places, 32 columns 16.8 / 11.5, 36 columns
+// 16.9 / 21.0; 8 of 2,000 35.6 / 29.7 and 36.2 / 36.8; 4 of 32,000 108.2 / 109.0 and 108.6 / 148.9.  A head of 256 leaves registers for half as many tiles.
 int tree_wide_tiles(int columns, int d) { return columns <= 32 ? 0 : d == 256 ? 2 : 4; }
 
 int tree_wide_launch(const TreeArgs& a, int d, hipStream_t stream) {
