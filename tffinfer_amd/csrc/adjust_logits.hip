@@ -11,8 +11,8 @@
 // history comes as it is, with repetitions, no table of counts by token has to be kept or cleared, counts are integers and so
 // do not depend on the order of the atomics.  Then it goes over its run once: what is masked is written and not read, and in place what no
 // option touches is neither.  The bound is memory: 4 bytes a logit in and out, of what a mask forbids only out.
-// us of the kernel, 151,936 logits a row: one row 4.2, 48 rows under grammars that allow one in fifty 13.8 (29 MB; a fill of as much takes 6.9, the
-// rest is the histories), 175 rows of trees, nine in ten allowed, 38 a call (4.6 TB/s).
+// us of the kernel, 151,936 logits a row: one row 4.4, 48 rows under grammars that allow one in fifty 13.8 (29 MB; a fill of as much takes 6.9, the
+// rest is the histories), 150 rows of trees, nine in ten allowed, 38 a call (4.6 TB/s).
 #include "common.h"
 #include "tffinfer_kernels.h"
 #include "tree_attention.h"
@@ -235,7 +235,7 @@ TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, 
     TFF_REQUIRE(cu_nodes || rows == requests, "adjust_logits: %d rows of %d requests", rows, requests);
     // Runs of 4,096 tokens, or of 2,048 where those would leave CUs with less than two blocks: every run goes through the request's whole history, so
     // few and long ones are better as soon as they fill the chip, and of the longer ones fewer are on a CU at a time.  us a call of 2,048 / 4,096 / 8,192:
-    // 48 rows of 151,936 logits, histories of up to 8,192 tokens 15.5 / 14.1 / 16.0, 175 rows of trees 44.2 / 38.2 / 45.3.
+    // 48 rows of 151,936 logits, histories of up to 8,192 tokens 15.5 / 14.1 / 16.0, 150 rows of trees 44.2 / 38.2 / 45.3.
     const int run = (int64_t)rows * ((V + 4095) / 4096) >= 2 * tff_device_cus() ? 4096 : 2048, runs = (V + run - 1) / run;
     TFF_REQUIRE((int64_t)rows * runs <= 0x7fffffff, "adjust_logits: %d rows of %d logits are more than a launch takes", rows, V);
     const AdjustArgs a{logits, out, rows, V, runs, history, cu_history, prompt_lens, history_len, requests, repetition, presence, frequency,

@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
 // scores' registers are the second product's operand as they lie.  The maximum that the exponentials are taken against follows the true one
 // when that is more than 2^8 ahead: the outputs are rescaled some times a run, not at every slice.  At a run's end the four waves meet in LDS; a
 // group of columns whose slices went to several blocks leaves a partial result with each, merged by a second kernel.
-// What bounds it: a few slices are latency (tables, pages, then the keys; 9.2 us for one request of 500 places and 26 columns, 1.3 MB), many the
+// What bounds it: a few slices are latency (tables, pages, then the keys; 8.7 us for one request of 300 places and 16 columns, 1.3 MB), many the
 // memory (4 requests of 32,000 places and 32 columns: 109 us, 4.8 TB/s).  float32 runs at its own MFMAs' rate, 2 us a slice and wave.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 tree_bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float tree_f32x4;
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
 
 // The partial results of a group of columns, in the order of the keys: a wave has H q heads of a node, and 8 / H partial results of each on their way
 // together.  A wave waits for memory four times one after the other, whatever it merges, so H is 4 where single heads would be more waves than the
-// GPU holds twice (870 nodes of 40 heads: 23.6 us with single heads, 18 so; 42 nodes of 16: 4.4, and 8).
+// GPU holds twice (874 nodes of 40 heads: 23.6 us with single heads, 18.3 so; 35 nodes of 16: 4.0, and 8).
 #define MERGE_HEADS 4
 template <typename T, int SLICE, int D, int COLS, int H>
 __global__ __launch_bounds__(256) void tree_merge_kernel(const TreeArgs a) {
