@@ -131,18 +131,16 @@ __device__ __forceinline__ int tree_wave_scan(int v) {
     return v;
 }
 
-// The weight of all requests, and of those before request `upto`; the same in every lane.
+// The weight of all requests; the same in every lane.
 template <int SLICE, int COLS>
-__device__ __forceinline__ void tree_units(const TreeArgs& a, int upto, int& total, int& before) {
-    total = before = 0;
+__device__ __forceinline__ int tree_total(const TreeArgs& a) {
+    int total = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         const int r = r0 + (int)(threadIdx.x & 63);
-        int u = 0;
-        if (r < a.R) u = tree_cost<SLICE, COLS>(tree_request<SLICE, COLS>(a, r));
-        const int incl = tree_wave_scan(u);
-        if (upto > r0) before += __builtin_amdgcn_readlane(incl, min(upto - r0, 64) - 1);
-        total += __builtin_amdgcn_readlane(incl, 63);
+        const int u = r < a.R ? tree_cost<SLICE, COLS>(tree_request<SLICE, COLS>(a, r)) : 0;
+        total += __builtin_amdgcn_readlane(tree_wave_scan(u), 63);
     }
+    return total;
 }
 // What a block takes: an equal share, and no less than `least` (a block has its loads to wait for before the first slice).
 __device__ __forceinline__ int tree_share(int total, int blocks, int least) { return max((total + blocks - 1) / blocks, least); }
@@ -165,8 +163,7 @@ template <int SLICE, int COLS>
 __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a, int b) {
     const int lane = threadIdx.x & 63;
     TreeRun run;
-    int total = 0, unused;
-    if (a.R > 64) tree_units<SLICE, COLS>(a, 0, total, unused);
+    int total = a.R > 64 ? tree_total<SLICE, COLS>(a) : 0;
     run.r = run.before = 0;
     for (int r0 = 0; r0 < a.R; r0 += 64) {
         TreeRequest t = tree_request<SLICE, COLS>(a, min(r0 + lane, a.R - 1));
