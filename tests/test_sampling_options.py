@@ -81,3 +81,22 @@ def test_command_line():
     assert cli.build_parser().parse_args(["m"]).logit_bias is None
     with pytest.raises(argparse.ArgumentTypeError):
         cli._parse_bias("5=1")
+
+
+class EmptyGrammar:
+    """Callable, and false where it stands empty: a grammar is there if it is given, whatever its truth value."""
+
+    def __init__(self):
+        self.stack = []
+
+    def __len__(self):
+        return len(self.stack)
+
+    def __call__(self, out):
+        return np.full(2, 5, dtype=np.uint32)
+
+
+def test_a_grammar_whose_truth_value_is_false():
+    c = SamplingConfig(allowed=EmptyGrammar())
+    assert not c.allowed and c.adjusts and c.needs_output
+    assert allowed_mask(c, np.zeros(0, np.int32), 40).tolist() == [5, 5]

@@ -60,12 +60,12 @@ class SamplingConfig:
     @property
     def adjusts(self) -> bool:
         """Whether the logits are changed by more than a repetition penalty."""
-        return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias or self.allowed)
+        return bool(self.presence_penalty or self.frequency_penalty or self.logit_bias) or self.allowed is not None
 
     @property
     def needs_output(self) -> bool:
         """Whether a token's choice depends on the tokens before it other than through the model."""
-        return bool(self.repetition_penalty != 1.0 or self.presence_penalty or self.frequency_penalty or self.allowed)
+        return bool(self.repetition_penalty != 1.0 or self.presence_penalty or self.frequency_penalty) or self.allowed is not None
 
     @property
     def greedy(self) -> bool:
