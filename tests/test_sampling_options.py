@@ -100,3 +100,15 @@ def test_a_grammar_whose_truth_value_is_false():
     c = SamplingConfig(allowed=EmptyGrammar())
     assert not c.allowed and c.adjusts and c.needs_output
     assert allowed_mask(c, np.zeros(0, np.int32), 40).tolist() == [5, 5]
+
+
+def test_options_that_float32_does_not_hold():
+    """They go to the device in float32, where 1e39 is infinite."""
+    most = float(np.finfo(np.float32).max)
+    for bad in (dict(presence_penalty=1e39), dict(presence_penalty=-1e39), dict(frequency_penalty=1e39), dict(frequency_penalty=-1e300),
+                dict(logit_bias={1: 1e39})):
+        with pytest.raises(ValueError):
+            SamplingConfig(**bad)
+    c = SamplingConfig(presence_penalty=-most, frequency_penalty=most, logit_bias={1: most, 2: -1e39, 3: -math.inf})
+    with np.errstate(over="ignore"):
+        assert np.asarray(list(c.logit_bias.values()), dtype=np.float32).tolist() == [most, -math.inf, -math.inf]

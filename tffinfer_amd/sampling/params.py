@@ -4,7 +4,6 @@ SamplingConfig (src/core/sampler/LLMSampler.h:55-63): ``_type``,
 ``_seed`` there, the same without the underscore here."""
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass, field
 from typing import Callable
 
@@ -12,6 +11,9 @@ import numpy as np
 
 #: strategy names of the reference (src/core/sampler/LLMSampler.h:18-24)
 STRATEGIES = ("default", "unknown", "greedy", "random", "top_k", "top_p")
+
+#: the device has the options in float32, where a larger number is infinite: a logit that it makes infinite has no softmax
+_FLOAT32_MAX = float(np.finfo(np.float32).max)
 
 
 @dataclass
@@ -48,14 +50,14 @@ class SamplingConfig:
             raise ValueError("top_k >= 0, 0 < top_p <= 1 and 0 <= min_p <= 1 are required")
         if self.repetition_penalty <= 0:
             raise ValueError("repetition_penalty must be positive")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
-            raise ValueError("presence_penalty and frequency_penalty must be numbers")
+        if not (abs(self.presence_penalty) <= _FLOAT32_MAX and abs(self.frequency_penalty) <= _FLOAT32_MAX):
+            raise ValueError("presence_penalty and frequency_penalty must be numbers of float32's range")
         if self.allowed is not None and not callable(self.allowed):
             raise ValueError("allowed must be a function of the output so far")
         if self.logit_bias is not None:
             self.logit_bias = {int(t): float(b) for t, b in self.logit_bias.items()}
-            if any(not b < math.inf for b in self.logit_bias.values()) or any(not 0 <= t < 1 << 31 for t in self.logit_bias):
-                raise ValueError("logit_bias: tokens must not be negative, biases numbers (or -inf, never again)")
+            if any(not b <= _FLOAT32_MAX for b in self.logit_bias.values()) or any(not 0 <= t < 1 << 31 for t in self.logit_bias):
+                raise ValueError("logit_bias: tokens must not be negative, biases numbers of float32's range (or -inf, never again)")
 
     @property
     def adjusts(self) -> bool:
