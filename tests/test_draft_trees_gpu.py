@@ -228,6 +228,48 @@ def test_attention_leaves_rows_that_no_request_has(nq, d):
     assert bool((out[32:] == 7.0).all()) and not bool((out[:32] == 7.0).all(1).any())
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("nodes, G", [(8, 8), (14, 8), (20, 8), (33, 8), (33, 5), (3, 16)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_of_many_columns_keeps_what_is_not_finite_to_those_who_see_it(d, nodes, G, bad):
+    """Groups of one to four tiles of columns a wave, whose waves share keys and values: what is not finite lies in the slice of keys that the nodes
+    begin in, in the last one, and in a cached place that the window passes for some nodes."""
+    rng = random.Random(nodes)
+    trees = [plain.random_tree(rng, nodes, 5) for _ in range(2)]
+    starts = [20, 100]
+
+    def poison(c):
+        for r, s in enumerate(starts):
+            for i, g, e in ((s + 1, 0, 3), (s + nodes - 1, 1, 5), (s - 18, 1, d - 1)):
+                c.values[r][i, g, e] = bad
+            if math.isnan(bad):
+                c.keys[r][s + 2, 0, 2] = bad
+            for i in (s + 1, s + nodes - 1, s - 18, s + 2):
+                c.put(r, i, c.keys[r][i], c.values[r][i])
+    check_attention(2 * G, 2, d, 16, BF16, starts, trees, poison=poison)
+    check_attention(2 * G, 2, d, 16, BF16, starts, trees, window=20, poison=poison, sinks=True)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("nodes", [5, 20, 33])
+def test_attention_of_many_columns_under_a_cap_and_with_sinks(d, nodes):
+    rng = random.Random(nodes)
+    for softcap, sinks, window in ((20.0, False, 0), (0.0, True, 0), (5.0, True, 0), (10.0, True, 40)):
+        check_attention(16, 2, d, 16, BF16, [90, 0, 300], some_trees(rng, [nodes, nodes, 3]), window=window, softcap=softcap, sinks=sinks)
+
+
+@pytest.mark.parametrize("nq, nkv, dtype, sizes", [(40, 8, BF16, (40, 7, 48, 1)), (18, 2, BF16, (60, 64, 57, 64)), (18, 2, F32, (60, 64, 57, 64)),
+                                                   (66, 1, BF16, (30, 9, 1, 25))])
+def test_attention_whose_merge_takes_four_heads_a_wave(nq, nkv, dtype, sizes):
+    """More than 16,384 (node, q head) pairs: a wave merges four heads, which lie in groups of columns of different numbers of partial results, beside heads
+    that are not there where nq is no multiple of four."""
+    rng = random.Random(nq)
+    sizes = [n for _ in range(4 if sum(sizes) > 200 else 5) for n in sizes]
+    starts = [rng.choice((0, 40, 130, 300, 700)) for _ in sizes]
+    assert sum(sizes) * nq > 16384
+    check_attention(nq, nkv, 64, 16, dtype, starts, some_trees(rng, sizes), sinks=nq == 18)
+
+
 def test_attention_window_of_any_size():
     q, k, v = (torch.randn(s, device=DEV).to(BF16) for s in ((3, 256), (4, 2, 16, 64), (4, 2, 64, 16)))
     args = (q, 4, 2, 64, k, v, ints([[3, 1, 0, 2]]), ints([0, 3]), ints([40]), ints([[1], [3], [5]]))
@@ -340,6 +382,29 @@ def test_adjust_rows_of_trees(V, n):
     for in_place in (False, True):
         check_adjust(4, V, [20, 0, 3, 0], [10, 0, 0, 0], PENS[2:], None, masks, [rng.randrange(-1, 2) for _ in range(rows)], trees, in_place)
         check_adjust(4, V, [20, 0, 3, 0], [10, 0, 0, 0], PENS[2:], [[(3, 1.0)], [], [(V - 1, -2.0)], []], trees=trees, in_place=in_place)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("R, V", [(40, 60001), (14, 151936)])
+def test_adjust_of_many_rows_of_a_real_vocabulary(R, V, in_place):
+    """Rows enough for runs of 4,096 logits, that begin anywhere, and a history that a block's threads go through in several turns, from an odd place on."""
+    rng = random.Random(V)
+    lens = [3, 10001, 0, 1, 4099] + [rng.randint(0, 60) for _ in range(R - 5)]
+    prompts = [rng.randint(0, n) for n in lens]
+    biases = [[(rng.randrange(V), rng.uniform(-5, 5)) for _ in range(rng.choice((0, 3, 300)))] for _ in lens]
+    masks = [list(range(V)), sorted(rng.sample(range(V), V // 50)), sorted(rng.sample(range(V), V - 5)), []]
+    pens = [PENS[r % 6] if r != 1 else (1.3, 0.5, 0.25) for r in range(R)]
+    check_adjust(R, V, lens, prompts, pens, biases, masks, [rng.randrange(-1, 4) for _ in lens], in_place=in_place)
+    check_adjust(R, V, lens, prompts, pens, in_place=in_place)
+
+
+def test_adjust_of_many_rows_of_trees():
+    rng = random.Random(12)
+    V, parents = 8193, [plain.random_tree(rng, n, 6) for n in (100, 50, 100)]
+    trees = [([rng.randrange(V) if rng.random() < 0.5 else rng.randrange(9) for _ in p], plain.paths(p)) for p in parents]
+    masks = [sorted(rng.sample(range(V), V // 2)), []]
+    for in_place in (False, True):
+        check_adjust(3, V, [20, 5000, 3], [10, 100, 0], PENS[2:5], None, masks, [rng.randrange(-1, 2) for _ in range(250)], trees, in_place)
 
 
 def test_adjust_leaves_rows_that_no_request_has():

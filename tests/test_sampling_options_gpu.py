@@ -101,3 +101,17 @@ def test_refusals(model_dirs):
     eng.add_request([1], SamplingConfig(allowed=lambda out: np.zeros(3, dtype=np.float32)))
     with pytest.raises(ValueError, match="allowed"):
         eng.step()
+
+
+def test_penalties_change_what_is_generated(model_dirs):
+    """A bias above any difference of two logits has one token come every time; a presence penalty above the two together lets none come twice, and a
+    frequency penalty of a third of the bias lets that one come three times before any other."""
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="float32", kv_tokens=256, max_num_seqs=3))
+    eng.keep_logits = True
+    one = {7: 300.0}
+    configs = [SamplingConfig(logit_bias=one), SamplingConfig(logit_bias=one, presence_penalty=1000.0),
+               SamplingConfig(logit_bias=one, frequency_penalty=100.0)]
+    same, once, thrice = eng.generate([[1, 2, 3]] * 3, configs, max_new_tokens=30, ignore_eos=True)
+    assert max(float(row.max() - row.min()) for r in (same, once, thrice) for row in r.logits) < 100.0
+    assert same.output == [7] * 30 and once.output[0] == 7 and len(set(once.output)) == 30
+    assert thrice.output[:3] == [7] * 3 and set(thrice.output) != {7}
