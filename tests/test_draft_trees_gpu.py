@@ -762,3 +762,25 @@ def test_two_streams_at_once():
     for i, want in enumerate(alone):
         for g in got[i]:
             assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+# ---- sinks that are not finite ----
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq, d", [(4, 64), (4, 80), (40, 128)])
+def test_attention_sinks_of_any_size(dtype, nq, d):
+    """A sink of -inf is none, one of +inf takes all the weight; where a node sees nothing the result is zeros whatever the sink, a NaN among them."""
+    n, starts, nkv, page = 5, [0, 40], 2, 16
+    k, v = (torch.randn(s, device=DEV).to(dtype) for s in ((8, nkv, page, d), (8, nkv, d, page)))
+    q, table, cu = torch.randn(2 * n, nq * d, device=DEV).to(dtype), ints(list(range(8)), (2, 4)), ints([0, n, 2 * n])
+    see = plain.packed([[], [0], [1, 2], [], [4]] * 2, 1).to(DEV)
+    args = (q, nq, nkv, d, k, v, table, cu, ints(starts), see)
+    none = ops.tree_attention(*args)
+    sinks = torch.full((nq,), -math.inf, device=DEV)
+    got = ops.tree_attention(*args, sinks=sinks)
+    assert bool((got[[0, 3]] == 0).all()) and torch.equal(got, none)
+    for x in (math.inf, math.nan, 1e30, -1e30):
+        got = ops.tree_attention(*args, sinks=torch.full((nq,), x, device=DEV))
+        assert bool((got[[0, 3]] == 0).all())
+        rest = torch.tensor([1, 2, 4, 5, 6, 7, 8, 9], device=DEV)
+        assert bool(torch.isnan(got[rest]).all()) if math.isnan(x) else bool((got[rest] == (0 if x > 0 else none[rest])).all())

@@ -82,10 +82,7 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
         }
     }
     T* op = out + ((size_t)t * nq + h) * d;
-    if (sinks) {                                 // one more term in the denominator, with no key and no value
-        const float ref = m == -INFINITY ? sinks[h] : m;
-        l += expf(sinks[h] - ref);
-    }
+    if (sinks) l += m == -INFINITY ? 1.f : expf(sinks[h] - m);      // one more term, with no key and no value (nothing seen: zeros, whatever the sink)
     const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
 #pragma unroll
     for (int i = 0; i < TREE_MAX_D / 64; ++i) {
