@@ -784,3 +784,27 @@ def test_attention_sinks_of_any_size(dtype, nq, d):
         assert bool((got[[0, 3]] == 0).all())
         rest = torch.tensor([1, 2, 4, 5, 6, 7, 8, 9], device=DEV)
         assert bool(torch.isnan(got[rest]).all()) if math.isnan(x) else bool((got[rest] == (0 if x > 0 else none[rest])).all())
+
+
+# ---- alignment ----
+
+@pytest.mark.parametrize("what", ["out", "q", "k", "v"])
+@pytest.mark.parametrize("nodes", [5, 30])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_of_tensors_that_begin_anywhere(what, nodes, dtype):
+    """An operand that begins at a multiple of its elements' size and no other is as good as any, and what lies before and behind the output stays."""
+    rng = random.Random(nodes)
+    nq, nkv, d, page, start = 8, 2, 64, 16, 70
+    c = Cache([start + nodes], nkv, d, page, dtype, 0.0)
+    t = dict(zip(("k", "v", "table"), c.gpu()))
+    t["q"] = torch.randn(nodes, nq * d, device=DEV).to(dtype)
+    t["out"] = torch.full((nodes, nq * d), 7.0, device=DEV, dtype=dtype)
+    room = torch.full((t[what].numel() + 2,), 7.0, device=DEV, dtype=dtype)
+    assert room.data_ptr() % 16 == 0
+    room[1:-1] = t[what].flatten()
+    t[what] = room[1:-1].view(t[what].shape)
+    see = plain.paths(plain.random_tree(rng, nodes, 6))
+    got = ops.tree_attention(t["q"], nq, nkv, d, t["k"], t["v"], t["table"], ints([0, nodes]), ints([start]), plain.packed(see, 1).to(DEV), out=t["out"])
+    assert got.data_ptr() == t["out"].data_ptr() and bool((room[[0, -1]] == 7.0).all())
+    o, o_abs, most = plain.attention(t["q"].cpu().view(nodes, nq, d), c.keys[0], c.values[0], start, see, nq, nkv)
+    assert bool(((got.cpu().double().view(nodes, nq, d) - o).abs() <= attention_tol(dtype, d, start + nodes, o, o_abs, most)).all())
