@@ -808,3 +808,52 @@ def test_attention_of_tensors_that_begin_anywhere(what, nodes, dtype):
     assert got.data_ptr() == t["out"].data_ptr() and bool((room[[0, -1]] == 7.0).all())
     o, o_abs, most = plain.attention(t["q"].cpu().view(nodes, nq, d), c.keys[0], c.values[0], start, see, nq, nkv)
     assert bool(((got.cpu().double().view(nodes, nq, d) - o).abs() <= attention_tol(dtype, d, start + nodes, o, o_abs, most)).all())
+
+
+# ---- the weights' sum ----
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq, d, nodes", [(4, 64, 5), (4, 128, 7), (8, 256, 3), (8, 64, 7), (16, 64, 30), (8, 128, 20), (16, 256, 12), (4, 80, 5)])
+def test_attention_of_equal_values_is_the_value(nq, d, nodes, dtype):
+    """Where all values of a head are one, so is the result, whatever the weights: their sum is that of the weights as the product has them, some of them
+    most of it.  In float32 product and sum go over up to 100 places, half a step of 2^-24 for each term and a few for the quotient; that is far from
+    half a step of bfloat16, where the result has the value's own bits."""
+    rng = random.Random(d)
+    for start in (0, 1, 9, 70):
+        c = Cache([start + nodes], 2, d, 16, dtype, 0.0, seed=start)
+        k, v, table = c.gpu()
+        v.copy_(torch.randn(2, d, device=DEV)[None, :, :, None].to(dtype).expand_as(v))
+        q = (3 * torch.randn(nodes, nq * d, device=DEV)).to(dtype)
+        see = plain.packed(plain.paths(plain.random_tree(rng, nodes, 6)), 1).to(DEV)
+        got = ops.tree_attention(q, nq, 2, d, k, v, table, ints([0, nodes]), ints([start]), see).view(nodes, 2, nq // 2, d)
+        want = v[0, :, :, 0][None, :, None].expand_as(got)
+        if dtype == BF16:
+            assert torch.equal(got, want), start
+        else:
+            assert bool(((got - want).abs() <= 2 * (start + nodes + 8) * 2.0 ** -24 * want.abs()).all()), start
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq, d, nodes", [(4, 64, 5), (4, 128, 7), (8, 256, 3), (16, 64, 30), (8, 128, 20), (4, 80, 5)])
+def test_attention_of_a_place_that_takes_most_of_the_weight(nq, d, nodes, dtype):
+    """A late place whose score is ahead of all before it, by less than a running maximum follows: its weight is some hundred, and rounds.  All values of a
+    head are one, which the result is, too, bound as above (2 * 160 half steps)."""
+    start, scores = 135, [-40.0] * 160
+    for seed in range(6):
+        rng = random.Random(seed)
+        for place in (5, 40, 70, 100):
+            scores[place] = 0.0
+        scores[130] = rng.uniform(4.0, 4.5)
+        k = torch.zeros(20, 2, 16, d, dtype=dtype)                   # (two tables' worth; the request has the first ten pages)
+        k[:10, :, :, 0] = torch.tensor(scores).view(10, 1, 16).to(dtype)
+        v = torch.randn(2, d).to(dtype)[None, :, :, None].expand(20, 2, d, 16).contiguous()
+        q = torch.zeros(nodes, nq, d, dtype=dtype)
+        q[:, :, 0] = (1.0 + 0.2 * torch.rand(nodes, nq)).to(dtype)
+        see = plain.packed(plain.paths(plain.random_tree(rng, nodes, 6)), 1).to(DEV)
+        got = ops.tree_attention(q.to(DEV).view(nodes, nq * d), nq, 2, d, k.to(DEV), v.to(DEV), ints(list(range(10)), (1, 10)), ints([0, nodes]),
+                                 ints([start]), see, scale=1.0).cpu().view(nodes, 2, nq // 2, d)
+        want = v[0, :, :, 0][None, :, None].expand_as(got)
+        if dtype == BF16:
+            assert torch.equal(got, want), seed
+        else:
+            assert bool(((got - want).abs() <= 2 * 160 * 2.0 ** -24 * want.abs()).all()), seed

@@ -124,10 +124,13 @@ struct TreeMath<bf16_t, D> {
         for (int f = 0; f < QF; ++f) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t * QF + f], q[f], s, 0, 0, 0);
         return s;
     }
+    // A weight as the product takes it: rounded to bfloat16, half a step of 2^-8.  The sum of the weights is that of the rounded ones, so that a dominant
+    // weight's rounding cancels.
+    static __device__ __forceinline__ float weight(float x) { return (float)(bf16_t)x; }
     static __device__ __forceinline__ void add(tree_f32x4 (&o)[D / 16], const frag (&v)[VF], const float (&p)[4 * TILES]) {
         frag w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = (bf16_t)p[i];       // (a weight rounds to bfloat16, half a step of 2^-8, as the product takes it)
+        for (int i = 0; i < 8; ++i) w[i] = (bf16_t)p[i];       // (they are bfloat16 numbers)
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt) o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[dt], w, o[dt], 0, 0, 0);
     }
@@ -186,6 +189,7 @@ struct TreeMath<float, D> {
             for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[f][e], q[f][e], s, 0, 0, 0);
         return s;
     }
+    static __device__ __forceinline__ float weight(float x) { return x; }
     static __device__ __forceinline__ void add(tree_f32x4 (&o)[D / 16], const frag (&v)[VF], const float (&p)[4 * TILES]) {
 #pragma unroll
         for (int dt = 0; dt < D / 16; ++dt)
@@ -411,7 +415,7 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
                 const float ref = m[ct] == -INFINITY ? 0.f : m[ct];
 #pragma unroll
                 for (int i = 0; i < KEYS; ++i) {
-                    p[ct][i] = __builtin_amdgcn_exp2f(p[ct][i] - ref);
+                    p[ct][i] = M::weight(__builtin_amdgcn_exp2f(p[ct][i] - ref));
                     l[ct] += p[ct][i];
                 }
             }
