@@ -857,3 +857,21 @@ def test_attention_of_a_place_that_takes_most_of_the_weight(nq, d, nodes, dtype)
             assert torch.equal(got, want), seed
         else:
             assert bool(((got - want).abs() <= 2 * 160 * 2.0 ** -24 * want.abs()).all()), seed
+
+
+# ---- a cap far above the scores ----
+
+@pytest.mark.parametrize("d", [64, 128, 256, 80])
+@pytest.mark.parametrize("softcap", [1.0, 50.0, 3e4])
+def test_attention_in_float32_holds_a_capped_score_by_its_own_size(d, softcap):
+    """c tanh(s / c) is off by some steps of the score, however large c is: a product, a quotient, tanh (two units in the last place, four half steps)
+    and two products more, 8 half steps of the largest |score| together, beside those of the score itself."""
+    n, nq, start = 9, 4, 60
+    see = plain.paths(plain.random_tree(random.Random(d), n, 5))
+    c = Cache([start + n], 2, d, 16, F32, 0.0, seed=d)
+    k, v, table = c.gpu()
+    q = torch.randn(n, nq * d)
+    got = ops.tree_attention(q.to(DEV), nq, 2, d, k, v, table, ints([0, n]), ints([start]), plain.packed(see, 1).to(DEV), softcap=softcap)
+    o, o_abs, most = plain.attention(q.view(n, nq, d), c.keys[0], c.values[0], start, see, nq, 2, softcap=softcap)
+    tol = attention_tol(F32, d, start + n, o, o_abs, most) + o_abs * 2 * 8 * 2.0 ** -24 * most
+    assert bool(((got.cpu().double().view(n, nq, d) - o).abs() <= tol).all())

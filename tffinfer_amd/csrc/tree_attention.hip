@@ -124,6 +124,12 @@ struct TreeMath<bf16_t, D> {
         for (int f = 0; f < QF; ++f) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t * QF + f], q[f], s, 0, 0, 0);
         return s;
     }
+    // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, whatever the score; for caps of some ten to a hundred less
+    // than a weight's rounding by far, as the attention of decoding has it in bfloat16
+    static __device__ __forceinline__ float capped(float x, float cap) {
+        const float e = __builtin_amdgcn_exp2f(-fabsf(x) * (2.f * 1.4426950408889634f / cap));
+        return copysignf(cap * (1.f - e) / (1.f + e), x);
+    }
     // A weight as the product takes it: rounded to bfloat16, half a step of 2^-8.  The sum of the weights is that of the rounded ones, so that a dominant
     // weight's rounding cancels.
     static __device__ __forceinline__ float weight(float x) { return (float)(bf16_t)x; }
@@ -189,6 +195,7 @@ struct TreeMath<float, D> {
             for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[f][e], q[f][e], s, 0, 0, 0);
         return s;
     }
+    static __device__ __forceinline__ float capped(float x, float cap) { return cap * tanhf(x / cap); }      // (a few steps of the score)
     static __device__ __forceinline__ float weight(float x) { return x; }
     static __device__ __forceinline__ void add(tree_f32x4 (&o)[D / 16], const frag (&v)[VF], const float (&p)[4 * TILES]) {
 #pragma unroll
@@ -370,15 +377,10 @@ __global__ __launch_bounds__(256, OCC) void tree_attention_kernel(const TreeArgs
                 }
             if (s + 4 < s1) load_k(s + 4, pk);
             if (a.softcap > 0.f) {
-                // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, as a score of its size is anyway
-                const float in = -2.f * a.scale / a.softcap * log2e, outer = a.softcap * log2e;
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(-fabsf(p[ct][i] * in)), h = outer * (1.f - e) / (1.f + e);
-                        p[ct][i] = copysignf(h, p[ct][i] * a.scale);
-                    }
+                    for (int i = 0; i < KEYS; ++i) p[ct][i] = M::capped(p[ct][i] * a.scale, a.softcap) * log2e;
             } else {
                 const float f = a.scale * log2e;
 #pragma unroll
