@@ -82,3 +82,8 @@ def test_host_tensors_are_refused():
     for call in calls:
         with pytest.raises(lib.KernelError, match="on the GPU"):
             call()
+
+
+def test_tree_attention_refuses_a_cap_that_is_infinite():
+    _refused("tff_tree_attention", {**ATTENTION, "softcap": float("inf")}.values(), "a cap of inf")
+    _refused("tff_tree_attention", {**ATTENTION, "softcap": float("nan")}.values(), "geometry")

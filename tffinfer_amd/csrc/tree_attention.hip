@@ -677,6 +677,7 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
     TFF_REQUIRE(d > 0 && d <= TREE_MAX_D, "tree_attention: head size %d not supported (1..%d)", d, TREE_MAX_D);
     TFF_REQUIRE(page_size > 0 && num_pages > 0 && bt_stride > 0 && window >= 0 && softcap >= 0.f,
                 "tree_attention: bad cache geometry page_size=%d pages=%d table stride=%d window=%d", page_size, num_pages, bt_stride, window);
+    TFF_REQUIRE(softcap < INFINITY, "tree_attention: a cap of %g (0: none)", (double)softcap);      // (times tanh(0), which is not a number)
     TFF_REQUIRE(words > 0 && words <= TREE_WORDS, "tree_attention: ancestors of %d words (1..%d)", words, TREE_WORDS);
     TFF_REQUIRE(q_stride >= nq * d, "tree_attention: query row stride %d below %d", q_stride, nq * d);
     TFF_REQUIRE(dtype == TFF_F32 || dtype == TFF_BF16, "tree_attention: unknown dtype %d", dtype);
