@@ -875,3 +875,40 @@ def test_attention_in_float32_holds_a_capped_score_by_its_own_size(d, softcap):
     o, o_abs, most = plain.attention(q.view(n, nq, d), c.keys[0], c.values[0], start, see, nq, 2, softcap=softcap)
     tol = attention_tol(F32, d, start + n, o, o_abs, most) + o_abs * 2 * 8 * 2.0 ** -24 * most
     assert bool(((got.cpu().double().view(n, nq, d) - o).abs() <= tol).all())
+
+
+# ---- node 0 and the history ----
+
+@pytest.mark.parametrize("V", [30, 5000])
+def test_adjust_rows_of_trees_are_rows_of_requests_that_have_their_path(V):
+    """What a request gets that has a node's path at its end, prompt and output in full and without a word of trees, the node's row gets: the same counts, so
+    the same bits.  Node 0 is the last token of a prompt of one token, of longer prompts, and of an output."""
+    rng = random.Random(V)
+    word = lambda: rng.randrange(min(V, 12))  # noqa: E731
+    cases = [(1, 0), (7, 0), (7, 1), (300, 40), (5, 9)]              # tokens of the prompt, of the output
+    have = [[word() for _ in range(p + o)] for p, o in cases]
+    trees = some_trees(rng, [6, 11, 1, 20, 33])
+    tokens = [h[-1:] + [word() for _ in t[1:]] for h, t in zip(have, trees)]
+    sees = [plain.paths(t) for t in trees]
+    rows = [(r, [tokens[r][j] for j in see]) for r, s in enumerate(sees) for see in s]
+    x = 3 * torch.randn(len(rows), V, device=DEV)
+    rep, pres, freq = ([rng.uniform(0.7, 1.6) for _ in cases], [rng.uniform(-1, 2) for _ in cases], [rng.uniform(-0.5, 1) for _ in cases])
+    bias = [[(word(), rng.uniform(-3, 3)) for _ in range(3)] for _ in cases]
+    f32 = lambda a: torch.tensor(a, dtype=F32, device=DEV)  # noqa: E731
+
+    def cu(lists):
+        return ints([sum(map(len, lists[:i])) for i in range(len(lists) + 1)])
+
+    def flat(lists):
+        return ints([y for s in lists for y in s])
+
+    def biases(lists):
+        return flat([[t for t, _ in s] for s in lists]), f32([b for s in lists for _, b in s]), cu(lists)
+    hist = [h[:-1] for h in have]
+    got = ops.adjust_logits(x, flat(hist), cu(hist), ints([p for p, _ in cases]), f32(rep), f32(pres), f32(freq), bias=biases(bias),
+                            drafts=(flat(tokens), cu(tokens), plain.packed([see for s in sees for see in s], 2).to(DEV)))
+    full = [hist[r] + path for r, path in rows]
+    each = lambda a: [a[r] for r, _ in rows]  # noqa: E731
+    want = ops.adjust_logits(x, flat(full), cu(full), ints([cases[r][0] for r, _ in rows]), f32(each(rep)), f32(each(pres)), f32(each(freq)),
+                             bias=biases(each(bias)))
+    assert torch.equal(got, want)

@@ -4,7 +4,8 @@
 //   x <- x - freq n_v - pres [n_v > 0]        n_v: how often v stands in its output
 //   x <- x + bias_v                           if v is listed
 //   x <- -inf                                 where the row's mask has no bit
-// The rows of drafted trees' nodes belong to the tree's request and have the tokens on their path (`ancestors`) as output besides.
+// The rows of drafted trees' nodes belong to the tree's request and have the tokens on their path (`ancestors`) as output besides: the history
+// ends before node 0, which is the request's last token and on every path (the prompt's, where the prompt is longer than the history).
 // The reference has the first of these, on the host (src/core/sampler/LLMSampler.cpp:21-34).
 //
 // A block takes a run of the vocabulary of one row and counts the tokens of the request's whole history that fall into it in LDS: the
@@ -77,6 +78,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
     }
     h0 = min(max(h0, 0), a.history_len);
     h1 = min(max(h1, h0), a.history_len);
+    const bool prompt_root = out0 > h1 - h0;      // (node 0 is the prompt's last token)
     out0 = h0 + min(max(out0, 0), h1 - h0);
     b0 = min(max(b0, 0), a.bias_len);
     b1 = min(max(b1, b0), a.bias_len);
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(256) void adjust_logits_kernel(const AdjustArgs a, 
         if (a.cu_nodes) {
             const int n0 = max(a.cu_nodes[r], 0), nodes = min(min(a.cu_nodes[r + 1], a.rows) - n0, 32 * a.words);
             for (int j = tid; j < nodes; j += 256)
-                if ((a.ancestors[(size_t)t * a.words + (j >> 5)] >> (j & 31)) & 1) count(a.draft_tokens[n0 + j], true);
+                if ((a.ancestors[(size_t)t * a.words + (j >> 5)] >> (j & 31)) & 1) count(a.draft_tokens[n0 + j], j > 0 || !prompt_root);
         }
         __syncthreads();
     }

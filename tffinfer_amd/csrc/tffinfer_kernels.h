@@ -622,7 +622,9 @@ TFF_API int tff_cache_keep(void* const* k_caches, void* const* v_caches, int num
 //   be null); then -inf where the row's mask lacks the token's bit: row mask_rows[t] of masks [num_masks, ceil(V / 32)], none
 //   where mask_rows[t] is no row of it (mask_rows may be null).
 // Row t is request t's, or with cu_nodes a node of a tree (above): its request's, with the tokens (draft_tokens [rows]) of the nodes
-// it sees as further output; rows from cu_nodes[requests] on are copied.  Token ids outside the vocabulary are passed over.
+// it sees as further output; rows from cu_nodes[requests] on are copied.  Node 0 is the last token that the request has and among what every path
+// sees, so with cu_nodes the history ends before it; where it is the prompt's, prompt_lens[r] is larger than the history, and it counts as prompt.
+// Token ids outside the vocabulary are passed over.
 TFF_API int tff_adjust_logits(const float* logits, float* out, int rows, int V, int requests, const int32_t* history, int history_len,
                               const int32_t* cu_history, const int32_t* prompt_lens, const float* repetition, const float* presence,
                               const float* frequency, const int32_t* bias_ids, const float* bias_values, int bias_len, const int32_t* cu_bias,

@@ -2656,7 +2656,10 @@ def adjust_logits(logits: torch.Tensor, history: torch.Tensor, cu_history: torch
     int32 cu [requests + 1]): numbers added to single tokens (of equal ones the last).  ``masks`` = (int32 [M, ceil(V / 32)],
     int32 [rows]): the tokens a row may choose, a bit each (lowest first), and the row's mask (-1: none); the others get -inf.
     ``drafts`` = (int32 tokens [rows], int32 cu_nodes [requests + 1], int32 ancestors [rows, words]): the rows are nodes of drafted trees
-    (:func:`tree_attention`) and have the tokens of the nodes they see as output, too; without it row i is request i's."""
+    (:func:`tree_attention`) and have the tokens of the nodes they see as output, too; without it row i is request i's.  Node 0 of a tree
+    is the last token its request has and is seen by every path, so with ``drafts`` the history ends *before* it.  Where it is the
+    prompt's last token, the history is the prompt without it and ``prompt_lens[r]`` the whole prompt's length, one more than the
+    history's: node 0 then counts as the prompt does."""
     what, i32, f32 = "adjust_logits", torch.int32, torch.float32
     dev = _place(logits, what)
     x = _operand(logits, dev, f32, 2, what, "logits")
