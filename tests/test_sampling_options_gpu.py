@@ -115,3 +115,36 @@ def test_penalties_change_what_is_generated(model_dirs):
     assert max(float(row.max() - row.min()) for r in (same, once, thrice) for row in r.logits) < 100.0
     assert same.output == [7] * 30 and once.output[0] == 7 and len(set(once.output)) == 30
     assert thrice.output[:3] == [7] * 3 and set(thrice.output) != {7}
+
+
+@pytest.mark.parametrize("how", ["raises", "wrong shape"])
+def test_a_grammar_that_fails_says_whose_it_is(model_dirs, how):
+    """The caller aborts that request, and the others end as they would have."""
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="float32", kv_tokens=256, max_num_seqs=3, page_size=8))
+    V = eng.model.config.vocab_size
+
+    def fine(out):
+        return packed(range(1, V, 2), V)
+
+    def grammar(out):
+        if len(out) < 4:
+            return packed(range(0, V, 3), V)
+        if how == "wrong shape":
+            return np.zeros(1, dtype=np.int32)
+        raise KeyError("no state")
+    prompts, kinds = [[1, 2, 3, 4, 5], [8, 9], [3]], [SamplingConfig(allowed=fine), SamplingConfig(allowed=grammar), SamplingConfig()]
+    want = [r.output for r in eng.generate([prompts[0], prompts[2]], [kinds[0], kinds[2]], max_new_tokens=12, ignore_eos=True)]
+    ids = [eng.add_request(p, c, 12, ignore_eos=True) for p, c in zip(prompts, kinds)]
+    failures = 0
+    while eng.has_work:
+        try:
+            eng.step()
+        except (ValueError, KeyError) as e:
+            failures += 1
+            assert e.request_id == ids[1]
+            eng.abort(ids[1])
+    assert failures == 1
+    assert [eng.pop_result(ids[0]).output, eng.pop_result(ids[2]).output] == want
+    r = eng.pop_result(ids[1])
+    assert len(r.output) == 4 and r.finish_reason != "length"
+    assert all(g.pool.num_used == 0 for g in eng.runner.cache.groups)

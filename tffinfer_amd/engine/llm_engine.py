@@ -219,13 +219,18 @@ class LLMEngine:
         histories = masks = None
         if any(r.sampling.adjusts for r in rows):
             histories = [self._history(r) if r.sampling.adjusts else None for r in rows]
+            masks, asked = [], None
             try:
                 # (before the step: a grammar that fails leaves the requests where they stood)
-                masks = [None if h is None else allowed_mask(r.sampling, h[0][h[1]:].copy(), self.model.config.vocab_size)
-                         for r, h in zip(rows, histories)]
-            except BaseException:
+                for asked, h in zip(rows, histories):
+                    masks.append(None if h is None else allowed_mask(asked.sampling, h[0][h[1]:].copy(), self.model.config.vocab_size))
+            except BaseException as e:
                 for p in plan:
                     self.runner.cache.rollback(p.request.id)
+                try:
+                    e.request_id = asked.id      # (whom to abort)
+                except AttributeError:           # (a frozen exception)
+                    pass
                 raise
         logits = self.runner.step(entries, token_source)
         if not rows:
@@ -316,7 +321,9 @@ class LLMEngine:
         """Plans and runs one step.  Returns (request id, new token, finished)
         for every request that got a token, and (request id, None, True) for a
         request that was dropped because the cache cannot hold it even alone
-        (finish reason "refused")."""
+        (finish reason "refused").  What a request's ``SamplingConfig.allowed``
+        raises comes through with the request's id as its ``request_id``, and
+        leaves all requests where they stood: :meth:`abort` that one and go on."""
         st = self._ahead
         self._ahead = None
         dropped = []
