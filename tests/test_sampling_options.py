@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tffinfer_amd import cli
-from tffinfer_amd.sampling import Sampler, SamplingConfig, TokenLog, allowed_mask
+from tffinfer_amd.sampling import Sampler, SamplingConfig, TokenLog, allowed_mask, allows_none
 
 
 def test_what_a_config_takes():
@@ -112,3 +112,18 @@ def test_options_that_float32_does_not_hold():
     c = SamplingConfig(presence_penalty=-most, frequency_penalty=most, logit_bias={1: most, 2: -1e39, 3: -math.inf})
     with np.errstate(over="ignore"):
         assert np.asarray(list(c.logit_bias.values()), dtype=np.float32).tolist() == [most, -math.inf, -math.inf]
+
+
+def test_masks_without_a_token():
+    """Bits behind the vocabulary are nobody's."""
+    for V in (1, 31, 32, 33, 64, 70):
+        words = -(-V // 32)
+        mask = np.zeros(words, dtype=np.int32)
+        assert allows_none(mask, V)
+        if V % 32:
+            mask[-1] = np.uint32(0xffffffff << (V % 32) & 0xffffffff).view(np.int32)
+            assert allows_none(mask, V)
+        for t in (0, V - 1):
+            one = mask.copy()
+            one.view(np.uint32)[t // 32] |= np.uint32(1 << (t % 32))
+            assert not allows_none(one, V), (V, t)

@@ -5,7 +5,7 @@ import torch
 
 import plain_draft_trees as plain
 from helpers import random_tokens
-from tffinfer_amd import EngineOptions, LLMEngine, SamplingConfig
+from tffinfer_amd import EngineOptions, LLMEngine, SamplingConfig, log
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,19 @@ def test_a_grammar_that_fails_says_whose_it_is(model_dirs, how):
     r = eng.pop_result(ids[1])
     assert len(r.output) == 4 and r.finish_reason != "length"
     assert all(g.pool.num_used == 0 for g in eng.runner.cache.groups)
+
+
+def test_a_grammar_that_allows_nothing_is_told(model_dirs):
+    """Token 0 stands where nothing was allowed; the result says where, the log says it once, and the other requests have nothing to tell."""
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="float32", kv_tokens=256, max_num_seqs=3))
+    V = eng.model.config.vocab_size
+
+    def dead_end(out):
+        return packed([] if len(out) in (2, 3, 5) else range(1, V), V)
+    before = log.counts()["W"]
+    configs = [SamplingConfig(allowed=dead_end), SamplingConfig(), SamplingConfig(allowed=lambda out: packed([V - 1], V)),
+               SamplingConfig("random", temperature=1.5, top_k=9, seed=4, allowed=dead_end), SamplingConfig("random", seed=5, allowed=dead_end)]
+    got = eng.generate([[1, 2], [3], [4], [5], [6]], configs, max_new_tokens=8, ignore_eos=True)
+    assert [r.unallowed for r in got] == [[2, 3, 5], [], [], [2, 3, 5], [2, 3, 5]]
+    assert all([i for i, t in enumerate(got[r].output) if t == 0] == [2, 3, 5] for r in (0, 3, 4)) and got[2].output == [V - 1] * 8
+    assert log.counts()["W"] == before + 3

@@ -12,9 +12,10 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
+from .. import log
 from ..kernels import staging as _staging
 from ..models import load_model
-from ..sampling import Sampler, SamplingConfig, SeenTokens, TokenLog, allowed_mask
+from ..sampling import Sampler, SamplingConfig, SeenTokens, TokenLog, allowed_mask, allows_none
 from .batch import StepEntry
 from .runner import ModelRunner
 from .scheduler import Request, Scheduler, SchedulerOptions
@@ -72,6 +73,7 @@ class GenerationResult:
     finish_reason: str
     num_preemptions: int = 0
     logits: list = field(default_factory=list)   # float32 rows at sampled positions, if kept
+    unallowed: list = field(default_factory=list)   # places of the output for which SamplingConfig.allowed left no token: token 0 is there
 
 
 def resolve_dtype(d) -> torch.dtype:
@@ -188,7 +190,7 @@ class LLMEngine:
             raise ValueError(f"request {request_id!r} has not finished")
         del self._requests[request_id]
         return GenerationResult(r.id, r.prompt, r.output, r.finish_reason, r.num_preemptions,
-                                self._results.pop(r.id, []))
+                                self._results.pop(r.id, []), [i for i in r.unallowed if i < len(r.output)])
 
     def abort(self, request_id) -> bool:
         return self.scheduler.abort(request_id)
@@ -223,7 +225,7 @@ class LLMEngine:
             try:
                 # (before the step: a grammar that fails leaves the requests where they stood)
                 for asked, h in zip(rows, histories):
-                    masks.append(None if h is None else allowed_mask(asked.sampling, h[0][h[1]:].copy(), self.model.config.vocab_size))
+                    masks.append(None if h is None else self._allowed(asked, h[0][h[1]:].copy()))
             except BaseException as e:
                 for p in plan:
                     self.runner.cache.rollback(p.request.id)
@@ -269,6 +271,16 @@ class LLMEngine:
         if log is None:
             log = req._token_log = TokenLog(req.prompt)
         return log.update(req.output), log.prompt_len
+
+    def _allowed(self, req, output):
+        """The request's mask for the token after ``output``; one without tokens is noted with the request."""
+        V = self.model.config.vocab_size
+        mask = allowed_mask(req.sampling, output, V)
+        if mask is not None and allows_none(mask, V) and output.size not in req.unallowed[-1:]:
+            if not req.unallowed:
+                log.warning("request %r: its grammar allows no token at place %d of the output, where token 0 is taken", req.id, output.size)
+            req.unallowed.append(output.size)
+        return mask
 
     def _complete(self, st: _Launched) -> list[tuple]:
         """Reads the step's tokens and tells the scheduler.  Requests that ended

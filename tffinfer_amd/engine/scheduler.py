@@ -67,6 +67,7 @@ class Request:
     status: str = "waiting"         # waiting | running | finished
     finish_reason: str | None = None
     num_preemptions: int = 0
+    unallowed: list = field(default_factory=list)   # places of the output for which its grammar allowed no token
 
     @property
     def tokens(self) -> list:

@@ -1,2 +1,2 @@
 from .params import STRATEGIES, SamplingConfig
-from .sampler import Sampler, SeenTokens, TokenLog, allowed_mask, uniform_at
+from .sampler import Sampler, SeenTokens, TokenLog, allowed_mask, allows_none, uniform_at

@@ -28,6 +28,17 @@ class SamplingConfig:
     positive and multiplies the other logits of tokens already in the prompt or
     the output (LLMSampler.cpp:21-34).  The draw for output token i of a
     request depends only on (seed, i), not on what else is in the batch.
+
+    ``presence_penalty`` comes off the logits of tokens in the output,
+    ``frequency_penalty`` as often as they stand there; ``logit_bias`` {token:
+    number} is added to single tokens' logits (-inf: never).  ``allowed`` is
+    called before every draw with the output so far (int32) and says what may
+    come next: int32 or uint32 [ceil(vocabulary / 32)], a bit a token, lowest
+    first, or None for all.  It may be called more than once for a place (a
+    step that failed runs again).  A mask without a single token leaves token
+    0, which it does not allow: the place is listed in the result's
+    ``unallowed`` and a warning logged.  A grammar that has come to its end
+    allows the stop token, or raises, which leaves the requests where they are.
     """
     type: str = "greedy"
     temperature: float = 1.0

@@ -82,6 +82,12 @@ def allowed_mask(config: SamplingConfig, output: np.ndarray, vocab: int) -> np.n
     return mask.view(np.int32)
 
 
+def allows_none(mask: np.ndarray, vocab: int) -> bool:
+    """Whether a mask (``allowed_mask``) has no bit for any of the ``vocab`` tokens."""
+    whole, rest = divmod(vocab, 32)
+    return not mask[:whole].any() and not (rest and int(mask[whole]) & ((1 << rest) - 1))
+
+
 class Sampler:
     def __init__(self, device, ops=_ops):
         self.device = device
