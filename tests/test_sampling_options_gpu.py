@@ -164,3 +164,18 @@ def test_a_grammar_that_allows_nothing_is_told(model_dirs):
     assert [r.unallowed for r in got] == [[2, 3, 5], [], [], [2, 3, 5], [2, 3, 5]]
     assert all([i for i, t in enumerate(got[r].output) if t == 0] == [2, 3, 5] for r in (0, 3, 4)) and got[2].output == [V - 1] * 8
     assert log.counts()["W"] == before + 3
+
+
+def test_only_who_needs_its_tokens_has_them_gathered(model_dirs):
+    """A bias alone asks for no history; a penalty and a grammar do."""
+    eng = LLMEngine.from_model_dir(model_dirs["A"], EngineOptions(dtype="float32", kv_tokens=256, max_num_seqs=4))
+    V = eng.model.config.vocab_size
+    asked, history = [], eng._history
+    eng._history = lambda r: asked.append(r.id) or history(r)
+    configs = [SamplingConfig(logit_bias={5: 50.0}), SamplingConfig(frequency_penalty=0.5), SamplingConfig(),
+               SamplingConfig(allowed=lambda out: packed([3], V))]
+    ids = [eng.add_request([1, 2], c, 3, ignore_eos=True) for c in configs]
+    while eng.has_work:
+        eng.step()
+    assert eng.pop_result(ids[0]).output == [5] * 3 and eng.pop_result(ids[3]).output == [3] * 3
+    assert sorted(asked) == sorted([ids[1], ids[3]] * 3)

@@ -220,12 +220,12 @@ class LLMEngine:
                 rows.append(p.request)
         histories = masks = None
         if any(r.sampling.adjusts for r in rows):
-            histories = [self._history(r) if r.sampling.adjusts else None for r in rows]
+            histories = [self._history(r) if r.sampling.adjusts and r.sampling.needs_output else None for r in rows]
             masks, asked = [], None
             try:
                 # (before the step: a grammar that fails leaves the requests where they stood)
                 for asked, h in zip(rows, histories):
-                    masks.append(None if h is None else self._allowed(asked, h[0][h[1]:].copy()))
+                    masks.append(None if asked.sampling.allowed is None else self._allowed(asked, h[0][h[1]:].copy()))
             except BaseException as e:
                 for p in plan:
                     self.runner.cache.rollback(p.request.id)
