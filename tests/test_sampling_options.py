@@ -127,3 +127,20 @@ def test_masks_without_a_token():
             one = mask.copy()
             one.view(np.uint32)[t // 32] |= np.uint32(1 << (t % 32))
             assert not allows_none(one, V), (V, t)
+
+
+def test_a_grammar_that_fills_one_array():
+    """Requests whose grammar hands out the same array, filled anew, have the mask that was theirs."""
+    got, room = [], np.zeros(2, dtype=np.int32)
+
+    def grammar(out):
+        room[:] = len(out)
+        return room
+    sampler = Sampler(torch.device("cpu"), types.SimpleNamespace(adjust_logits=lambda *a, **kw: got.append(kw["masks"]), argmax=lambda x: x))
+    c = SamplingConfig(allowed=grammar)
+    histories = [(np.arange(n, dtype=np.int32), 1) for n in (4, 2, 7)]
+    sampler.sample_on_device(torch.zeros(3, 40), [c] * 3, [0] * 3, None, histories)
+    given = [allowed_mask(c, h[0][h[1]:], 40) for h in histories]
+    sampler.sample_on_device(torch.zeros(3, 40), [c] * 3, [0] * 3, None, histories, given)
+    for masks, rows in got:
+        assert masks.tolist() == [[3, 3], [1, 1], [6, 6]] and rows.tolist() == [0, 1, 2]

@@ -72,11 +72,12 @@ class TokenLog:
 
 
 def allowed_mask(config: SamplingConfig, output: np.ndarray, vocab: int) -> np.ndarray | None:
-    """What the config's ``allowed`` says about the token after ``output``: int32 [ceil(vocab / 32)], or None for all."""
+    """What the config's ``allowed`` says about the token after ``output``: int32 [ceil(vocab / 32)], or None for all.  A copy: the
+    function may fill the same array again for the next request."""
     mask = config.allowed(output) if config.allowed is not None else None
     if mask is None:
         return None
-    mask = np.ascontiguousarray(mask)
+    mask = np.array(mask, order="C")
     if mask.dtype not in (np.int32, np.uint32) or mask.shape != (-(-vocab // 32),):
         raise ValueError(f"allowed() returned {mask.dtype} {mask.shape}, expected int32 or uint32 {(-(-vocab // 32),)}")
     return mask.view(np.int32)
