@@ -8,7 +8,7 @@
 // From node 0 (the token the request already had) on: to the first child whose token is what the model chose after the node, until no
 // child is or `max_path` nodes are kept.  A node's parent is the last node that it sees before itself.  A wave a request: a lane
 // has the nodes lane, lane + 64, ..., and a level is a comparison and a ballot.  Bound by latency: two loads after each other, then
-// registers (2.2 us for one request of 8 nodes, 3.6 for 64 of up to 64).
+// registers (2.2 us for one request of 8 nodes, 3.9 for 64 of up to 64).
 __global__ __launch_bounds__(64) void tree_accept_kernel(const int32_t* __restrict__ choices, const int32_t* __restrict__ tokens,
                                                          const int32_t* __restrict__ cu_nodes, const int32_t* __restrict__ ancestors,
                                                          int words, int T, int max_path, int32_t* __restrict__ path,

@@ -12,7 +12,9 @@
 #define TREE_MAX_D 512
 
 // ---- any head size, page size and type: a wave per (node, q head), keys 64 at a time, one a lane ----
-// The yardstick, and what sizes run on that the matrix cores' kernel does not take.
+// The yardstick, and what sizes run on that the matrix cores' kernel does not take.  It reads a kv head's keys and values once per node and q head of
+// the group, each lane a key of its own: one request of 300 places and 16 columns 105 us with a head of 80, 152 with one of 192; 8 of 2,048 and 104 columns
+// 2,250 (heads of 64 and 128 on the matrix cores: 9.2; 30 and 36).
 template <typename T>
 __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
     const T* __restrict__ q, int q_stride, T* __restrict__ out, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
@@ -102,8 +104,9 @@ __global__ __launch_bounds__(64) void tree_attention_generic_kernel(
 // scores' registers are the second product's operand as they lie.  The maximum that the exponentials are taken against follows the true one
 // when that is more than 2^8 ahead: the outputs are rescaled some times a run, not at every slice.  At a run's end the four waves meet in LDS; a
 // group of columns whose slices went to several blocks leaves a partial result with each, merged by a second kernel.
-// What bounds it: a few slices are latency (tables, pages, then the keys; 8.7 us for one request of 300 places and 16 columns, 1.3 MB), many the
-// memory (4 requests of 32,000 places and 32 columns: 109 us, 4.8 TB/s).  float32 runs at its own MFMAs' rate, 2 us a slice and wave.
+// What bounds it: a few slices are latency, some 4.5 us until a run's first keys are there (tables, pages, keys) and 1.5 for every slice that a wave has
+// (one request and 16 columns: 40 places, a slice a wave, 6.0 us, 150 7.4, 300 9.2, 480 10.8); many are the memory (4 requests of 32,000 places and 32
+// columns, 524 MB: 102 us and a merge of 7, 4.8 TB/s).  float32 runs at its own MFMAs' rate, 2 us a slice and wave.
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 tree_bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float tree_f32x4;
 typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t tree_u32x4;
@@ -659,7 +662,10 @@ static TreePlan tree_plan(int rows, int R, int nq, int nkv, int d, int page_size
     long long blocks = (long long)tff_device_cus() * per_cu / nkv;
     if (blocks < 1) blocks = 1;
     if (blocks > (units + p.least - 1) / p.least) blocks = (units + p.least - 1) / p.least;
-    p.blocks = !p.wide && dtype == TFF_BF16 && units <= 16 ? 1 : (int)blocks;      // (what one block has whole needs no merge)
+    // Tables of up to 512 places: what one block has whole needs no merge.  us of the kernels, one request and 16 columns, so / on several blocks: 40 places
+    // 6.0 / 6.2 + 3.1, 150 7.4 / 7.6 + 3.0, 300 9.1 / 9.1 + 3.2, 480 10.8 / 8.1 + 5.0.  The lengths are the device's, so a wider table has the second
+    // form whatever they are: 300 places under a table of 2,560 pages 9.3 + 3.1.
+    p.blocks = !p.wide && dtype == TFF_BF16 && units <= 16 ? 1 : (int)blocks;
     return p;
 }
 TFF_API size_t tff_tree_attention_workspace_bytes(int rows, int R, int nq, int nkv, int d, int page_size, int bt_stride, int dtype) {

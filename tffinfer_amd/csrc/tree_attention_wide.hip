@@ -9,8 +9,8 @@
 // reduce a maximum nor rescale.  The sum of a column's weights is one more row of the second product (values of one): it is the sum of the
 // weights as they are rounded, so that a dominant weight's rounding cancels.
 // What bounds it: with 256 columns and a head of 128 the issue of a wave's 68 MFMAs, 32 exponentials and some 130 other instructions a
-// slice; with fewer columns the keys and values from memory.  4 requests of 32,700 places (543 MB): 64 columns 113 us (4.8 TB/s, what a
-// copy reads and writes), 128 126, 192 141, 256 166 (717 TFLOP/s; the copies alone take 118, the arithmetic alone 135).
+// slice, one wave a SIMD (the MFMAs are busy for two fifths of the time); with fewer columns the keys and values from memory.  us of the kernel for 4
+// requests of 32,000 places (524 MB): 64 columns 101 (5.2 TB/s), 128 116, 192 136, 256 158 (847 TFLOP/s); the merges take 6 to 11 more.
 #include <type_traits>
 #include <utility>
 
@@ -195,7 +195,8 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
             }
         };
         auto cap = [&](floatx4 (&x)[NT][2]) INLINE {
-            // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, as a score of its size is anyway
+            // c tanh(x / c) = c (1 - e) / (1 + e), e = e^(-2 |x| / c): off by about half a step of c, whatever the score; for caps of some ten to a
+            // hundred less than a weight's rounding by far
             const float in = -2.f * fabsf(a.scale) / a.softcap * log2e, outer = a.softcap * log2e;
 #pragma unroll
             for (int ct = 0; ct < NT; ++ct) {
@@ -550,8 +551,9 @@ __global__ __launch_bounds__(256, 1) void tree_wide_kernel(const TreeArgs a) {
 
 }  // namespace
 
-// Up to 32 columns all waves have all of them (tree_attention.hip): us here / there, one request of 200 places, 32 columns 16.8 / 11.5, 36 columns
-// 16.9 / 21.0; 8 of 2,000 35.6 / 29.7 and 36.2 / 36.8; 4 of 32,000 108.2 / 109.0 and 108.6 / 148.9.  A head of 256 leaves registers for half as many tiles.
+// Up to 32 columns all waves have all of them (tree_attention.hip): us of the kernels, merge included, here / there, pages of 64: one request of 200
+// places, 32 columns 17.4 / 10.8, 36 columns 17.5 / 17.8; 8 of 2,000 33.6 / 30.9 and 34.5 / 35.9; 4 of 32,000 105 / 111 and 104 / 150.  A head of 256
+// leaves registers for half as many tiles.
 int tree_wide_tiles(int columns, int d) { return columns <= 32 ? 0 : d == 256 ? 2 : 4; }
 
 int tree_wide_launch(const TreeArgs& a, int d, hipStream_t stream) {
