@@ -694,11 +694,11 @@ TFF_API int tff_tree_attention(const void* q, int q_stride, void* out, const voi
     const int esz = dtype == TFF_F32 ? 4 : 2;
     const uintptr_t q0 = (uintptr_t)q, q1 = q0 + (size_t)rows * q_stride * esz, o0 = (uintptr_t)out, o1 = o0 + (size_t)rows * nq * d * esz;
     TFF_REQUIRE(o1 <= q0 || q1 <= o0, "tree_attention: the output overlaps the queries");      // (a block reads queries after others have written)
+    const TreePlan p = tree_plan(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
     const size_t need = tff_tree_attention_workspace_bytes(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
     if (need > 0 && workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0 && ((uintptr_t)q & 15) == 0 &&
         ((size_t)q_stride * esz) % 16 == 0 && ((uintptr_t)k_cache & 15) == 0 && ((uintptr_t)v_cache & 15) == 0 &&
-        ((uintptr_t)out & 7) == 0) {      // (the kernel of many columns stores 8 bytes at a time)
-        const TreePlan p = tree_plan(rows, R, nq, nkv, d, page_size, bt_stride, dtype);
+        (!p.wide || ((uintptr_t)out & 7) == 0)) {      // (the kernel of many columns stores 8 bytes at a time)
         int shift = 3;
         for (int i = 3; i < 31; ++i)
             if (page_size == 1 << i) shift = i;
