@@ -144,3 +144,11 @@ def test_a_grammar_that_fills_one_array():
     sampler.sample_on_device(torch.zeros(3, 40), [c] * 3, [0] * 3, None, histories, given)
     for masks, rows in got:
         assert masks.tolist() == [[3, 3], [1, 1], [6, 6]] and rows.tolist() == [0, 1, 2]
+
+
+def test_biases_below_float32s_range_are_never():
+    """They become -inf where they are given; a cast at every step would warn of an overflow at every step."""
+    c = SamplingConfig(logit_bias={2: -1e39, 3: -math.inf, 4: -1e38})
+    assert c.logit_bias == {2: -math.inf, 3: -math.inf, 4: -1e38}
+    with np.errstate(over="raise"):
+        assert np.asarray(list(c.logit_bias.values()), dtype=np.float32)[0] == -math.inf

@@ -4,6 +4,7 @@ SamplingConfig (src/core/sampler/LLMSampler.h:55-63): ``_type``,
 ``_seed`` there, the same without the underscore here."""
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from typing import Callable
 
@@ -69,6 +70,7 @@ class SamplingConfig:
             self.logit_bias = {int(t): float(b) for t, b in self.logit_bias.items()}
             if any(not b <= _FLOAT32_MAX for b in self.logit_bias.values()) or any(not 0 <= t < 1 << 31 for t in self.logit_bias):
                 raise ValueError("logit_bias: tokens must not be negative, biases numbers of float32's range (or -inf, never again)")
+            self.logit_bias = {t: b if b >= -_FLOAT32_MAX else -math.inf for t, b in self.logit_bias.items()}
 
     @property
     def adjusts(self) -> bool:
