@@ -105,8 +105,8 @@ class Sampler:
         row r decides (the counter of its random draw); ``seen[r]`` the tokens
         of its prompt and output so far (needed only with a repetition penalty):
         a sequence, or its distinct tokens as an int32 array (``SeenTokens``).
-        ``histories[r]`` is (prompt and output as an int32 array, tokens of the prompt), for rows whose
-        config says ``adjusts`` (``TokenLog``); ``masks[r]`` is ``allowed_mask`` of the row (asked for here where not given).
+        ``histories[r]`` is (prompt and output as an int32 array, tokens of the prompt), for rows whose config says ``adjusts``
+        and ``needs_output`` (``TokenLog``); ``masks[r]`` is ``allowed_mask`` of the row (asked for here where not given).
         ``logits`` may be changed in place by the options."""
         if logits.shape[0] == 0:
             return []
